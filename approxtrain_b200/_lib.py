@@ -17,6 +17,8 @@ DETERMINISTIC = 1
 INT32 = 2
 ACT_NONE, ACT_RELU = 0, 1
 STATIC_SCRATCH_BYTES = 8 << 20
+NORM_RMS, NORM_POST, NORM_PRE = 1, 2, 4
+NORM_MAX_WIDTH = 32768
 
 # every symbol include/amsim.h declares
 EXPORTS = [
@@ -29,6 +31,7 @@ EXPORTS = [
     "amsim_matmul_ex", "amsim_bias_grad_workspace", "amsim_bias_grad",
     "amsim_debug_fastdiv", "amsim_debug_launch_count", "amsim_debug_reload_env", "amsim_debug_bounds_report",
     "amsim_async_status", "amsim_debug_wait_report",
+    "amsim_residual_norm", "amsim_residual_norm_grad_workspace", "amsim_residual_norm_grad",
 ]
 
 
@@ -83,6 +86,11 @@ def _load() -> C.CDLL:
     L.amsim_debug_wait_report.argtypes = [C.POINTER(C.c_uint)]
     L.amsim_debug_reload_env.argtypes = []
     L.amsim_debug_reload_env.restype = None
+    ll, f = C.c_longlong, C.c_float
+    L.amsim_residual_norm.argtypes = [vp] * 11 + [ll, ip, ll, f, f, ip, ip, ip, u]
+    L.amsim_residual_norm_grad_workspace.argtypes = [ll, ip, ip, ip, u]
+    L.amsim_residual_norm_grad_workspace.restype = sz
+    L.amsim_residual_norm_grad.argtypes = [vp] * 17 + [ll, ip, ll, f, ip, ip, ip, vp, sz, u]
     return L
 
 

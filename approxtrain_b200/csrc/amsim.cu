@@ -26,8 +26,10 @@
 #include "amsim_codes.cuh"
 #include "amsim_codes_launch.h"
 #include "amsim_factor.h"
+#include "amsim_host.h"
 #ifndef AMSIM_SPLIT_TU
 #include "amsim_codes.cu"
+#include "amsim_norm.cu"
 #endif
 
 #include <atomic>
@@ -224,6 +226,25 @@ int report_stuck(int device) {
   if (!take_stuck(device)) return AMSIM_OK;
   return fail(AMSIM_ERR_CUDA, "a tensor-core kernel of an earlier call gave up waiting between its warps: the results of that call are wrong");
 }
+
+}  // namespace
+
+namespace amsim {
+
+int host_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+void host_count_launch() { AMSIM_COUNT_LAUNCH(); }
+int host_sm_count(int device) { return sm_count(device); }
+int host_device() { return current_device(); }
+
+}  // namespace amsim
+
+namespace {
 
 // approx_mul_lut.h:22-25
 int parse_mant_width(const char* path) {

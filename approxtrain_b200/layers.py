@@ -23,8 +23,10 @@ import os
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
+from .train_ops import _NormArgs, _norm_forward
 
 
 class GradSink:
@@ -385,3 +387,59 @@ class BatchNormNHWC(nn.BatchNorm2d):
 
     def forward(self, x):
         return super().forward(x.permute(0, 3, 1, 2)).permute(0, 2, 3, 1)
+
+
+# ---- exact operators of the library around the products ---------------------------------------
+class _ResidualNormFn(torch.autograd.Function):
+    """(sum, norm) of ops.residual_norm.  The backward pass makes the normalised rows again from x, the block
+    and the rows' statistics."""
+
+    @staticmethod
+    def forward(ctx, x, block, gate, post_w, post_b, pre_w, pre_b, args, need_sum):
+        r, y, stats = _norm_forward(args, need_sum, True)
+        ctx.save_for_backward(args.x, stats, args.block, args.gate, args.post_w, args.post_b, args.pre_w, args.pre_b)
+        ctx.cfg = (args.gate_rows, args.scale, args.flags)
+        ctx.set_materialize_grads(False)
+        return r, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dy):
+        x, stats, block, gate, post_w, post_b, pre_w, pre_b = ctx.saved_tensors
+        gate_rows, scale, flags = ctx.cfg
+        dr, dy = (None if g is None else g.contiguous() for g in (dr, dy))
+        grads = ops.residual_norm_grad(dr, dy, x, stats, block, gate, gate_rows, scale, post_w, post_b, pre_w, pre_b, flags,
+                                       wants=ctx.needs_input_grad[:7])
+        return (*(g if want else None for g, want in zip(grads, ctx.needs_input_grad)), None, None)
+
+
+def residual_norm(x, block=None, gate=None, scale=1.0, post=None, pre=None, kind="layer", eps=1e-3, need_sum=True):
+    """``ops.residual_norm`` with gradients for x, block, gate, weights and biases."""
+    args = _NormArgs(x, block, gate, scale, post, pre, kind, eps)
+    leaves = (x, block, gate, *(post or (None, None)), *(pre or (None, None)))
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves)):
+        return _norm_forward(args, need_sum, False)[:2]
+    r, y = _ResidualNormFn.apply(*leaves, args, need_sum or not args.pre)
+    return r, y
+
+
+class ResidualNorm(nn.Module):
+    """The norms around a residual block: ``(x, block) -> (x + scale * gate * N_post(block), N_pre of that)``.  ``post_norm`` /
+    ``pre_norm`` say which norms there are, ``gate_init`` (a number) makes the gate a parameter of one value per column.
+    With ``post_norm=False`` and no gate it is "add & norm" of the reference's Transformer (ammha/encoder.py, decoder.py)."""
+
+    def __init__(self, width, kind="layer", post_norm=False, pre_norm=True, gate_init=None, scale=1.0, eps=1e-3):
+        super().__init__()
+        self.kind, self.scale, self.eps = kind, scale, eps
+        self.has_post, self.has_pre = post_norm, pre_norm
+        for name, on in (("post", post_norm), ("pre", pre_norm)):
+            self.register_parameter(name + "_weight", nn.Parameter(torch.ones(width)) if on else None)
+            self.register_parameter(name + "_bias", nn.Parameter(torch.zeros(width)) if on and kind == "layer" else None)
+        self.gate = nn.Parameter(torch.full((width,), float(gate_init))) if gate_init is not None else None
+
+    def forward(self, x, block=None, need_sum=True):
+        with_block = block is not None
+        return residual_norm(x, block, gate=self.gate if with_block else None, scale=self.scale,
+                             post=(self.post_weight, self.post_bias) if self.has_post and with_block else None,
+                             pre=(self.pre_weight, self.pre_bias) if self.has_pre else None, kind=self.kind, eps=self.eps,
+                             need_sum=need_sum)

@@ -1,0 +1,186 @@
+"""Operators of a Transformer training step around the table products.
+
+=====================  ==================================================================
+``residual_norm``      norms before and after a block with its gate and residual scale
+=====================  ==================================================================
+
+Same manner as :mod:`approxtrain_b200.ops`, which exports all of them: torch CUDA tensors, one call into ``libamsim.so``
+on the current stream, no CPU implementation.  The functions here compute; :mod:`approxtrain_b200.layers` wires the
+gradients.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._lib import lib, check, NORM_RMS, NORM_POST, NORM_PRE, NORM_MAX_WIDTH
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _tensor(t, name: str, like: torch.Tensor = None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device: there is no CPU implementation")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    return t
+
+
+def _call(device: torch.device, fn, *args) -> None:
+    """``fn(current stream, ...)`` with `device` current; raises what the library reports."""
+    idx = device.index
+    if idx == torch.cuda.current_device():
+        check(fn(torch._C._cuda_getCurrentRawStream(idx), *args))
+    else:
+        with torch.cuda.device(idx):
+            check(fn(torch._C._cuda_getCurrentRawStream(idx), *args))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---- residual_norm --------------------------------------------------------------------------------
+def _norm_pair(pair, name, x):
+    """(present, weight, bias) of a norm given as None, (weight, bias) or (None, None)."""
+    if pair is None:
+        return False, None, None
+    w, b = pair
+    out = []
+    for t, part in ((w, "weight"), (b, "bias")):
+        if t is not None:
+            t = _tensor(t, f"{name} {part}", x)
+            if tuple(t.shape) != (x.shape[-1],):
+                raise ValueError(f"{name} {part} must have shape [{x.shape[-1]}], got {list(t.shape)}")
+            t = t.contiguous()
+        out.append(t)
+    return True, out[0], out[1]
+
+
+def _gate_rows(gate, x) -> int:
+    """Rows of the gate: 1 for [width], else the leading axes it shares with x (the rest of them 1)."""
+    width = x.shape[-1]
+    if gate.dim() == 1 and gate.shape[0] == width:
+        return 1
+    bad = f"gate must have shape [{width}], x's shape {list(x.shape)}, or that with trailing row axes of 1, got {list(gate.shape)}"
+    if gate.dim() != x.dim() or gate.shape[-1] != width:
+        raise ValueError(bad)
+    rows, shared = 1, True
+    for g, n in zip(gate.shape[:-1], x.shape[:-1]):
+        shared = shared and g == n
+        if shared:
+            rows *= g
+        elif g != 1:
+            raise ValueError(bad)
+    return rows
+
+
+class _NormArgs:
+    """Checked arguments of residual_norm, contiguous."""
+
+    def __init__(self, x, block, gate, scale, post, pre, kind, eps):
+        x = _tensor(x, "x")
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise ValueError(f"x must have at least one column, got shape {list(x.shape)}")
+        if x.shape[-1] > NORM_MAX_WIDTH:
+            raise ValueError(f"rows of at most {NORM_MAX_WIDTH} elements, got {x.shape[-1]}")
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"kind must be 'layer' or 'rms', got {kind!r}")
+        if not eps >= 0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        self.x = x.contiguous()
+        self.block = self.gate = None
+        if block is not None:
+            block = _tensor(block, "block", x)
+            if block.shape != x.shape or block.dtype != x.dtype:
+                raise ValueError(f"block must match x ({x.dtype}, {list(x.shape)}), got {block.dtype}, {list(block.shape)}")
+            self.block = block.contiguous()
+        elif post is not None or gate is not None:
+            raise ValueError("a norm after the block or a gate needs a block")
+        self.gate_rows = 0
+        self.width = x.shape[-1]
+        self.rows = x.numel() // self.width
+        if gate is not None:
+            self.gate_rows = _gate_rows(_tensor(gate, "gate", x), x)
+            self.gate = gate.contiguous()
+        has_post, self.post_w, self.post_b = _norm_pair(post, "post", x)
+        has_pre, self.pre_w, self.pre_b = _norm_pair(pre, "pre", x)
+        if not has_pre and block is None:
+            raise ValueError("neither a block to add nor a norm to take")
+        if kind == "rms" and (self.post_b is not None or self.pre_b is not None):
+            raise ValueError("rms norms have no bias")
+        w_types = {t.dtype for t in (self.post_w, self.post_b, self.pre_w, self.pre_b) if t is not None}
+        if len(w_types) > 1:
+            raise TypeError(f"weights and biases must have one type, got {sorted(str(t) for t in w_types)}")
+        self.w_type = _TYPES[w_types.pop()] if w_types else 0
+        self.type = _TYPES[x.dtype]
+        self.gate_type = _TYPES[self.gate.dtype] if self.gate is not None else 0
+        if self.w_type not in (0, self.type) or self.gate_type not in (0, self.type):
+            raise TypeError("weights, biases and gate must be float32 or have x's type")
+        self.scale, self.eps = float(scale), float(eps)
+        self.pre = has_pre
+        self.flags = (NORM_RMS if kind == "rms" else 0) | (NORM_POST if has_post else 0) | (NORM_PRE if has_pre else 0)
+
+
+def _norm_forward(a: _NormArgs, need_sum: bool, need_stats: bool):
+    r = torch.empty_like(a.x) if need_sum or not a.pre else None
+    y = torch.empty_like(a.x) if a.pre else None
+    stats = torch.empty((a.rows, 4), dtype=torch.float32, device=a.x.device) if need_stats else None
+    _call(a.x.device, lib.amsim_residual_norm, a.x.data_ptr(), _ptr(a.block), _ptr(a.gate), _ptr(a.post_w), _ptr(a.post_b),
+          _ptr(a.pre_w), _ptr(a.pre_b), _ptr(r), _ptr(y), _ptr(stats), a.rows, a.width, a.gate_rows, a.scale, a.eps, a.type,
+          a.w_type, a.gate_type, a.flags)
+    return r, y, stats
+
+
+def residual_norm(x, block=None, gate=None, scale: float = 1.0, post=None, pre=None, kind: str = "layer", eps: float = 1e-3,
+                  need_sum: bool = True):
+    """The norms around a residual block in one launch:
+
+    ``u = norm(block; post)`` or ``block``; ``r = x + scale * gate * u``; ``y = norm(r; pre)``; returns ``(r, y)``.
+
+    ``post`` (the norm after the block) and ``pre`` (the norm before the next block) are ``(weight, bias)``, either of
+    which may be None, or None for no such norm (``y`` is then None).  ``kind``: "layer" norms subtract the mean,
+    "rms" norms do not and have no bias.  ``gate``: [width], or x's shape with any number of its trailing row axes 1
+    (``[batch, 1, width]``: one per sequence).  x, block: float32, bfloat16 or float16, any leading axes, rows of up to
+    32768 elements; weights, biases, gate: float32 or x's type.  Computed in FP32, every output rounded once.
+    ``need_sum=False``: ``r`` is not written and returned as None.  For gradients use ``layers.residual_norm``."""
+    r, y, _ = _norm_forward(_NormArgs(x, block, gate, scale, post, pre, kind, eps), need_sum, False)
+    return r, y
+
+
+def residual_norm_grad(dr, dy, x, stats, block=None, gate=None, gate_rows: int = 0, scale: float = 1.0, post_w=None, post_b=None,
+                       pre_w=None, pre_b=None, flags: int = NORM_PRE, wants=(True,) * 7):
+    """Gradients (x, block, gate, post weight, post bias, pre weight, pre bias) of ``residual_norm`` from those of its
+    outputs (either may be None); ``stats`` is the forward pass's, ``wants`` says which are computed.  The sum is made
+    again from x and block, unrounded.  Where x and block are only added (no norm after the block, no gate, scale 1) the block's gradient is x's tensor."""
+    like = x
+    rows, width = (like.numel() // like.shape[-1], like.shape[-1])
+    post, pre = bool(flags & NORM_POST), bool(flags & NORM_PRE)
+    device = like.device
+    dx = torch.empty_like(like)
+    plain = not post and gate is None and scale == 1.0
+    dblock = torch.empty_like(like) if wants[1] and not plain else None
+    dgate = torch.empty_like(gate) if gate is not None and wants[2] else None
+
+    def grad_of(p, want):
+        return torch.empty_like(p) if p is not None and want else None
+    dpost_w, dpost_b, dpre_w, dpre_b = (grad_of(p, w) for p, w in zip((post_w, post_b, pre_w, pre_b), wants[3:]))
+    weights = next((t for t in (post_w, post_b, pre_w, pre_b) if t is not None), None)
+    if dr is None and dy is None:
+        for t in (dx, dblock, dgate, dpost_w, dpost_b, dpre_w, dpre_b):
+            if t is not None:
+                t.zero_()
+    else:
+        with torch.cuda.device(device):
+            size = lib.amsim_residual_norm_grad_workspace(rows, width, gate is not None, _TYPES[like.dtype], flags)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        _call(device, lib.amsim_residual_norm_grad, _ptr(dr), _ptr(dy), x.data_ptr(), _ptr(block), _ptr(gate), _ptr(post_w), _ptr(post_b),
+              _ptr(pre_w), stats.data_ptr(), dx.data_ptr(), _ptr(dblock), _ptr(dgate), _ptr(dpost_w), _ptr(dpost_b), _ptr(dpre_w),
+              _ptr(dpre_b), rows, width, gate_rows, scale, _TYPES[like.dtype], _TYPES[weights.dtype] if weights is not None else 0,
+              _TYPES[gate.dtype] if gate is not None else 0, ws.data_ptr() if size else None, size, flags)
+    if wants[1] and plain:
+        dblock = dx
+    return dx, dblock, dgate, dpost_w, dpost_b, dpre_w, dpre_b

@@ -290,6 +290,40 @@ size_t amsim_bias_grad_workspace(long long rows, int cols);
 int amsim_bias_grad(void* stream, const float* grad, float* dbias, long long rows, int cols,
                     void* workspace, size_t workspace_bytes);
 
+/* ---- the norms around a residual block -----------------------------------------------
+ * (No reference counterpart; in its networks these are stock LayerNormalization and add ops.)
+ *     u = N_post(block) or block;  sum = x + scale * gate * u;  y = N_pre(sum)
+ * over rows of `width` elements; N is a layer norm (mean and deviation, weight and bias) or, with AMSIM_NORM_RMS, x / rms(x)
+ * times a weight.  `block`, `gate`, the weights and biases may be NULL (no block: sum = x).  AMSIM_NORM_POST / _PRE
+ * say which norms there are; with neither a weight nor a bias a norm is plain.  `gate` has gate_rows rows of
+ * `width`; rows / gate_rows consecutive rows share one.  Types (x, block, sum, y: `dtype`): AMSIM_F32, AMSIM_BF16, AMSIM_F16;
+ * weights and biases (w_dtype) and gate (gate_dtype) are AMSIM_F32 or dtype.  Everything is computed in FP32 and rounded once.  `sum` may
+ * be NULL where only y is wanted, `stats` (rows x 4 floats, 16-byte aligned) where no gradient will be taken. */
+#define AMSIM_F32 0
+#define AMSIM_BF16 1
+#define AMSIM_F16 2
+#define AMSIM_NORM_RMS 1u
+#define AMSIM_NORM_POST 2u
+#define AMSIM_NORM_PRE 4u
+#define AMSIM_NORM_MAX_WIDTH 32768
+int amsim_residual_norm(void* stream, const void* x, const void* block, const void* gate,
+                        const void* post_w, const void* post_b, const void* pre_w,
+                        const void* pre_b, void* sum, void* y, float* stats, long long rows,
+                        int width, long long gate_rows, float scale, float eps, int dtype,
+                        int w_dtype, int gate_dtype, unsigned flags);
+/* Its gradient.  `dsum` or `dy` may be NULL (no gradient for that output); x, block, gate and weights are the forward call's
+ * (the sum is made again from them, unrounded), and so is `stats`.  `dx` is written always; `dblock` and the gradients of
+ * gate, weights and biases where not NULL.  Without N_post and gate and with scale 1, dblock equals dx.  Sums over rows run in a fixed order: the same bits on every run. */
+size_t amsim_residual_norm_grad_workspace(long long rows, int width, int has_gate, int dtype,
+                                          unsigned flags);
+int amsim_residual_norm_grad(void* stream, const void* dsum, const void* dy, const void* x,
+                             const void* block, const void* gate, const void* post_w,
+                             const void* post_b, const void* pre_w, const float* stats, void* dx,
+                             void* dblock, void* dgate, void* dpost_w, void* dpost_b, void* dpre_w,
+                             void* dpre_b, long long rows, int width, long long gate_rows,
+                             float scale, int dtype, int w_dtype, int gate_dtype, void* workspace,
+                             size_t workspace_bytes, unsigned flags);
+
 /* Number of kernels this library has launched since it was loaded (all devices, all
  * streams).  For benchmarks that report their launch count; no reference counterpart. */
 unsigned long long amsim_debug_launch_count(void);

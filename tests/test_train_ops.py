@@ -1,0 +1,88 @@
+"""Refusals of the operators around the table products; no kernel is launched."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def L():
+    from approxtrain_b200 import _build
+    _build.build()
+    from approxtrain_b200 import _lib
+    return _lib
+
+
+def test_residual_norm_refuses_cpu_tensors_and_other_types(L):
+    from approxtrain_b200 import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.residual_norm(torch.zeros(2, 4), torch.zeros(2, 4), pre=(None, None))
+    with pytest.raises(TypeError):
+        ops.residual_norm([1.0], pre=(None, None))
+
+
+def _norm(L, x=1 << 20, block=1 << 21, gate=None, w=(None,) * 4, r=1 << 22, y=1 << 23, stats=None, rows=4, width=8, gate_rows=0,
+          scale=1.0, eps=1e-3, types=(0, 0, 0), flags=4):
+    """The C entry point with made-up addresses: every call here is refused before anything is launched."""
+    return L.lib.amsim_residual_norm(None, x, block, gate, *w, r, y, stats, rows, width, gate_rows, scale, eps, *types, flags)
+
+
+def test_residual_norm_abi_refusals(L):
+    p = 1 << 24
+    assert _norm(L, flags=8) == L.ERR_INVALID and b"flag" in L.lib.amsim_last_error()
+    assert _norm(L, rows=-1) == L.ERR_INVALID
+    assert _norm(L, width=0) == L.ERR_INVALID
+    assert _norm(L, width=L.NORM_MAX_WIDTH + 1) == L.ERR_UNSUPPORTED
+    assert _norm(L, rows=1 << 40) == L.ERR_UNSUPPORTED
+    assert _norm(L, types=(3, 0, 0)) == L.ERR_INVALID
+    assert _norm(L, types=(0, 1, 0)) == L.ERR_INVALID
+    assert _norm(L, types=(1, 1, 2)) == L.ERR_INVALID
+    assert _norm(L, gate=p, gate_rows=3) == L.ERR_INVALID
+    assert _norm(L, gate=p, gate_rows=0) == L.ERR_INVALID
+    assert _norm(L, block=None, gate=p, gate_rows=1) == L.ERR_INVALID
+    assert _norm(L, block=None, flags=6) == L.ERR_INVALID
+    assert _norm(L, w=(None, None, None, p), flags=5) == L.ERR_INVALID       # an rms norm's bias
+    assert _norm(L, eps=-1.0) == L.ERR_INVALID
+    assert _norm(L, eps=float("nan")) == L.ERR_INVALID
+    assert _norm(L, flags=0, r=None) == L.ERR_INVALID
+    assert _norm(L, x=None) == L.ERR_INVALID
+    assert _norm(L, y=None) == L.ERR_INVALID
+    assert _norm(L, stats=p + 4) == L.ERR_INVALID
+    assert _norm(L, rows=0) == 0
+
+
+def test_residual_norm_grad_abi_refusals(L):
+    p = 1 << 24
+
+    def call(dsum=p, dy=p, r=p, block=p, gate=None, w=(None,) * 3, stats=p, dx=p, dblock=None, dgate=None, dw=(None,) * 4, rows=4,
+             width=8, gate_rows=0, ws=p, ws_bytes=1 << 30, flags=4):
+        return L.lib.amsim_residual_norm_grad(None, dsum, dy, r, block, gate, *w, stats, dx, dblock, dgate, *dw, rows, width, gate_rows,
+                                              1.0, 0, 0, 0, ws, ws_bytes, flags)
+    assert call(dsum=None, dy=None) == L.ERR_INVALID
+    assert call(dx=None) == L.ERR_INVALID
+    assert call(stats=None) == L.ERR_INVALID
+    assert call(r=None) == L.ERR_INVALID
+    assert call(flags=6, block=None) == L.ERR_INVALID
+    assert call(dgate=p) == L.ERR_INVALID
+    assert call(dw=(p, None, None, None)) == L.ERR_INVALID                   # no norm after the block
+    assert call(flags=0) == L.ERR_INVALID                                    # a gradient of a norm that there is not
+    assert call(flags=5, dw=(None, None, None, p)) == L.ERR_INVALID
+    assert call(ws=None) == L.ERR_WORKSPACE
+    assert call(ws_bytes=16) == L.ERR_WORKSPACE
+    assert call(ws=p + 8) == L.ERR_WORKSPACE
+    assert L.lib.amsim_residual_norm_grad_workspace(0, 8, 0, 0, 4) == 0
+    assert L.lib.amsim_residual_norm_grad_workspace(1000, 8, 1, 0, 4) > L.lib.amsim_residual_norm_grad_workspace(1000, 8, 0, 0, 4) > 0
+
+
+def test_gate_shapes():
+    from approxtrain_b200.train_ops import _gate_rows
+    x = torch.zeros(3, 5, 7, 4)
+    assert _gate_rows(torch.zeros(4), x) == 1
+    assert _gate_rows(torch.zeros(1, 1, 1, 4), x) == 1
+    assert _gate_rows(torch.zeros(3, 1, 1, 4), x) == 3
+    assert _gate_rows(torch.zeros(3, 5, 1, 4), x) == 15
+    assert _gate_rows(x, x) == 105
+    for bad in ((3,), (1, 5, 1, 4), (3, 1, 7, 4), (3, 5, 7, 1), (5, 4), (3, 2, 1, 4)):
+        with pytest.raises(ValueError, match="gate"):
+            _gate_rows(torch.zeros(bad), x)
