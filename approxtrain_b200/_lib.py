@@ -19,6 +19,7 @@ ACT_NONE, ACT_RELU = 0, 1
 STATIC_SCRATCH_BYTES = 8 << 20
 NORM_RMS, NORM_POST, NORM_PRE = 1, 2, 4
 NORM_MAX_WIDTH = 32768
+ROTARY_INTERLEAVED, ROTARY_INVERSE, ROTARY_POS32 = 1, 2, 4
 
 # every symbol include/amsim.h declares
 EXPORTS = [
@@ -32,6 +33,7 @@ EXPORTS = [
     "amsim_debug_fastdiv", "amsim_debug_launch_count", "amsim_debug_reload_env", "amsim_debug_bounds_report",
     "amsim_async_status", "amsim_debug_wait_report",
     "amsim_residual_norm", "amsim_residual_norm_grad_workspace", "amsim_residual_norm_grad",
+    "amsim_rotary",
 ]
 
 
@@ -91,6 +93,7 @@ def _load() -> C.CDLL:
     L.amsim_residual_norm_grad_workspace.argtypes = [ll, ip, ip, ip, u]
     L.amsim_residual_norm_grad_workspace.restype = sz
     L.amsim_residual_norm_grad.argtypes = [vp] * 17 + [ll, ip, ll, f, ip, ip, ip, vp, sz, u]
+    L.amsim_rotary.argtypes = [vp, vp, vp, ip, vp, vp, ip, vp, vp, ll, ll, ip, ip, C.POINTER(ll), f, ip, u]
     return L
 
 

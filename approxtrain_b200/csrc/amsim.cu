@@ -30,6 +30,7 @@
 #ifndef AMSIM_SPLIT_TU
 #include "amsim_codes.cu"
 #include "amsim_norm.cu"
+#include "amsim_rotary.cu"
 #endif
 
 #include <atomic>

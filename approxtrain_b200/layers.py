@@ -443,3 +443,34 @@ class ResidualNorm(nn.Module):
                              post=(self.post_weight, self.post_bias) if self.has_post and with_block else None,
                              pre=(self.pre_weight, self.pre_bias) if self.has_pre else None, kind=self.kind, eps=self.eps,
                              need_sum=need_sum)
+
+
+class _RotaryFn(torch.autograd.Function):
+    """ops.rotary; a rotation's gradient is the rotation back."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, layout):
+        ctx.save_for_backward(positions)
+        ctx.cfg = (freqs, layout)
+        ctx.set_materialize_grads(False)
+        return ops.rotary(q, positions, freqs, k=k, layout=layout)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        positions, = ctx.saved_tensors
+        freqs, layout = ctx.cfg
+        if dq is None:
+            dk = ops.rotary(dk, positions, freqs, layout=layout, inverse=True) if dk is not None else None
+        elif dk is None:
+            dq = ops.rotary(dq, positions, freqs, layout=layout, inverse=True)
+        else:
+            dq, dk = ops.rotary(dq, positions, freqs, k=dk, layout=layout, inverse=True)
+        return dq, dk, None, None, None
+
+
+def rotary(q, positions, freqs, k=None, layout="half"):
+    """``ops.rotary`` with gradients for q and k."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(q, k, positions, freqs, layout)
+    return ops.rotary(q, positions, freqs, k=k, layout=layout)

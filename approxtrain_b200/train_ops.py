@@ -2,6 +2,7 @@
 
 =====================  ==================================================================
 ``residual_norm``      norms before and after a block with its gate and residual scale
+``rotary``             rotary positions of queries and keys
 =====================  ==================================================================
 
 Same manner as :mod:`approxtrain_b200.ops`, which exports all of them: torch CUDA tensors, one call into ``libamsim.so``
@@ -10,9 +11,12 @@ gradients.
 """
 from __future__ import annotations
 
+import ctypes as C
+import math
+
 import torch
 
-from ._lib import lib, check, NORM_RMS, NORM_POST, NORM_PRE, NORM_MAX_WIDTH
+from ._lib import lib, check, NORM_RMS, NORM_POST, NORM_PRE, NORM_MAX_WIDTH, ROTARY_INTERLEAVED, ROTARY_INVERSE, ROTARY_POS32
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -184,3 +188,111 @@ def residual_norm_grad(dr, dy, x, stats, block=None, gate=None, gate_rows: int =
     if wants[1] and plain:
         dblock = dx
     return dx, dblock, dgate, dpost_w, dpost_b, dpre_w, dpre_b
+
+
+# ---- rotary ---------------------------------------------------------------------------------------
+class RotaryFrequencies:
+    """Angles per position of the rotated pairs (float64, on the device) and the factor on the rotated values."""
+
+    def __init__(self, inv_freq: torch.Tensor, scale: float = 1.0):
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.numel() == 0:
+            raise TypeError("inv_freq must be a float64 tensor of one frequency per pair")
+        if not inv_freq.is_cuda:
+            raise ValueError("inv_freq must live on a CUDA device: there is no CPU implementation")
+        self.inv_freq = inv_freq.contiguous()
+        self.scale = float(scale)
+        self.rotary_dim = 2 * inv_freq.numel()
+
+
+def _frequencies64(rotary_dim, base, scaling, factor, original_length, low_turns, high_turns):
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
+    if not base > 0 or not factor > 0:
+        raise ValueError("base and factor must be positive")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f, scale = base ** (-2.0 * i / rotary_dim), 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "blend":
+        if not original_length > 0 or not high_turns > low_turns:
+            raise ValueError("scaling 'blend' needs original_length > 0 and high_turns > low_turns")
+        keep = ((original_length * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1 - keep)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"scaling must be None, 'linear', 'base' or 'blend', got {scaling!r}")
+    return f, scale
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling=None, factor: float = 1.0, original_length: int = 0,
+                       low_turns: float = 1.0, high_turns: float = 32.0, device="cuda") -> RotaryFrequencies:
+    """The frequencies ``base ** (-2 i / rotary_dim)``, scaled for contexts `factor` times as long:
+
+    ``"linear"``  every frequency divided by `factor` (positions interpolated);
+    ``"base"``    the base raised by ``factor ** (rotary_dim / (rotary_dim - 2))``, which divides the lowest by `factor`;
+    ``"blend"``   frequencies that turn more than `high_turns` times over `original_length` stay, those below `low_turns` are
+                  divided by `factor`, linearly between, and rotated values are multiplied by ``0.1 ln(factor) + 1``."""
+    f, scale = _frequencies64(rotary_dim, base, scaling, factor, original_length, low_turns, high_turns)
+    return RotaryFrequencies(f.to(device), scale)
+
+
+def _rotary_heads(x, name, like=None):
+    x = _tensor(x, name, like)
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [batch, positions, heads, dim] or [positions, heads, dim], got {list(x.shape)}")
+    if like is not None and (x.dim() != like.dim() or x.dtype != like.dtype or x.shape[:-2] != like.shape[:-2] or x.shape[-1] != like.shape[-1]):
+        raise ValueError(f"{name} must match the first tensor's type, batch, positions and dim, got {x.dtype}, {list(x.shape)}")
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _strides(x):
+    return (0, *x.stride()[:2]) if x.dim() == 3 else x.stride()[:3]
+
+
+_StrideArray = C.c_longlong * 14
+
+
+def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half", inverse: bool = False, inplace: bool = False):
+    """Rotary positions of q (and k): pair i of a head at position p turns by ``p * freqs.inv_freq[i]``.
+
+    q, k: [batch, positions, heads, dim] or [positions, heads, dim], float32, bfloat16 or float16, any strides with a dense
+    last axis (``transpose(1, 2)`` of [batch, heads, positions, dim], a slice of a joint projection); k may have other heads
+    than q.  ``positions``: int32 or int64, [positions] or [batch, positions].  ``layout``: "half" (pairs half of the rotated
+    part apart) or "interleaved" (adjacent).  The first ``freqs.rotary_dim`` elements of a head turn, the rest are
+    copied.  ``inverse`` turns back.  ``inplace`` writes over q and k.  Returns q's result, or both."""
+    q = _rotary_heads(q, "q") if not inplace else _tensor(q, "q")
+    k_ = None
+    if k is not None:
+        k_ = _rotary_heads(k, "k", q)
+    if inplace:
+        for t, name in ((q, "q"), (k, "k")):
+            if t is not None and t.shape[-1] != 1 and t.stride(-1) != 1:
+                raise ValueError(f"{name} must have a dense last axis to be rotated in place")
+            if t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{name} must not be an expanded tensor to be rotated in place")
+        _rotary_heads(q, "q")
+    if not isinstance(freqs, RotaryFrequencies):
+        raise TypeError("freqs must be RotaryFrequencies (rotary_frequencies)")
+    if freqs.rotary_dim > q.shape[-1]:
+        raise ValueError(f"{freqs.rotary_dim} rotated elements in heads of {q.shape[-1]}")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 tensor")
+    if positions.device != q.device or freqs.inv_freq.device != q.device:
+        raise ValueError(f"positions and frequencies must be on {q.device}")
+    batch = q.shape[0] if q.dim() == 4 else 1
+    seq = q.shape[-3]
+    if tuple(positions.shape) not in ((seq,), (batch, seq)):
+        raise ValueError(f"positions must have shape [{seq}] or [{batch}, {seq}], got {list(positions.shape)}")
+    out = q if inplace else torch.empty_like(q)
+    out2 = (k_ if inplace else torch.empty_like(k_)) if k_ is not None else None
+    ps = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    none = (0, 0, 0)
+    strides = _StrideArray(*_strides(q), *_strides(out), *(_strides(k_) if k_ is not None else none), *(_strides(out2) if k_ is not None else none), *ps)
+    flags = (ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (ROTARY_INVERSE if inverse else 0) | (ROTARY_POS32 if positions.dtype == torch.int32 else 0)
+    _call(q.device, lib.amsim_rotary, q.data_ptr(), out.data_ptr(), q.shape[-2], _ptr(k_), _ptr(out2), k_.shape[-2] if k_ is not None else 0,
+          positions.data_ptr(), freqs.inv_freq.data_ptr(), batch, seq, q.shape[-1], freqs.rotary_dim, strides, freqs.scale, _TYPES[q.dtype], flags)
+    return out if k is None else (out, out2)

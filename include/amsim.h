@@ -324,6 +324,23 @@ int amsim_residual_norm_grad(void* stream, const void* dsum, const void* dy, con
                              float scale, int dtype, int w_dtype, int gate_dtype, void* workspace,
                              size_t workspace_bytes, unsigned flags);
 
+/* ---- rotary positions -----------------------------------------------------------------
+ * (No reference counterpart: its Transformer adds sinusoids to the embeddings, ammha/positional_encoding.py.)
+ * Rotates the first `rotary_dim` elements of every head of x (and of x2, may be NULL with heads2 0; both share positions and
+ * frequencies): pair i at position p turns by p * freqs[i] and is multiplied by `scale`; elements behind them are copied.  Pairs are
+ * half of the rotated part apart, or adjacent with AMSIM_ROTARY_INTERLEAVED; AMSIM_ROTARY_INVERSE turns back (the
+ * gradient).  Angles are taken in 64 bits.  `freqs`: rotary_dim / 2 doubles on the device.  `positions`: int64 (int32
+ * with AMSIM_ROTARY_POS32) on the device.  `strides` (host, elements): batch, position and head of x, of out, of x2, of
+ * out2; batch and position of `positions` (0 to share).  The last axis is dense.  out == x with equal strides works in
+ * place; outputs that overlap their inputs otherwise are not allowed. */
+#define AMSIM_ROTARY_INTERLEAVED 1u
+#define AMSIM_ROTARY_INVERSE 2u
+#define AMSIM_ROTARY_POS32 4u
+int amsim_rotary(void* stream, const void* x, void* out, int heads, const void* x2, void* out2,
+                 int heads2, const void* positions, const double* freqs, long long batch,
+                 long long seq, int dim, int rotary_dim, const long long* strides, float scale,
+                 int dtype, unsigned flags);
+
 /* Number of kernels this library has launched since it was loaded (all devices, all
  * streams).  For benchmarks that report their launch count; no reference counterpart. */
 unsigned long long amsim_debug_launch_count(void);

@@ -86,3 +86,34 @@ def test_gate_shapes():
     for bad in ((3,), (1, 5, 1, 4), (3, 1, 7, 4), (3, 5, 7, 1), (5, 4), (3, 2, 1, 4)):
         with pytest.raises(ValueError, match="gate"):
             _gate_rows(torch.zeros(bad), x)
+
+
+def test_rotary_refusals(L):
+    from approxtrain_b200 import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.rotary(torch.zeros(1, 2, 1, 8), torch.arange(2), None)
+    for kw in (dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, scaling="other"),
+               dict(rotary_dim=8, scaling="blend"), dict(rotary_dim=8, scaling="linear", factor=-1.0)):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(device="cpu", **kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.RotaryFrequencies(torch.ones(4, dtype=torch.float64))
+    with pytest.raises(TypeError):
+        ops.RotaryFrequencies(torch.ones(4))
+    p = 1 << 20
+    strides = (C.c_longlong * 14)(64, 16, 8, 64, 16, 8, 64, 16, 8, 64, 16, 8, 0, 1)
+
+    def call(x=p, out=2 * p, heads=2, x2=None, out2=None, heads2=0, pos=p, freqs=p, batch=1, seq=4, dim=8, rot=8, st=strides, dtype=0, flags=0):
+        return L.lib.amsim_rotary(None, x, out, heads, x2, out2, heads2, pos, freqs, batch, seq, dim, rot, st, 1.0, dtype, flags)
+    assert call(flags=8) == L.ERR_INVALID
+    assert call(dtype=3) == L.ERR_INVALID
+    assert call(batch=-1) == L.ERR_INVALID
+    assert call(rot=0) == L.ERR_INVALID and call(rot=7) == L.ERR_INVALID and call(rot=10) == L.ERR_INVALID
+    assert call(dim=20000, rot=20000) == L.ERR_UNSUPPORTED
+    assert call(batch=1 << 31) == L.ERR_UNSUPPORTED
+    assert call(batch=1 << 21, seq=1 << 21) == L.ERR_UNSUPPORTED
+    assert call(x=None) == L.ERR_INVALID and call(pos=None) == L.ERR_INVALID and call(freqs=None) == L.ERR_INVALID and call(st=None) == L.ERR_INVALID
+    assert call(heads2=1) == L.ERR_INVALID
+    other = (C.c_longlong * 14)(64, 16, 8, 64, 16, 4, 0, 0, 0, 0, 0, 0, 0, 1)
+    assert call(out=p, st=other) == L.ERR_INVALID and b"in place" in L.lib.amsim_last_error()
+    assert call(batch=0) == 0 and call(heads=0) == 0
