@@ -33,7 +33,7 @@ EXPORTS = [
     "amsim_debug_fastdiv", "amsim_debug_launch_count", "amsim_debug_reload_env", "amsim_debug_bounds_report",
     "amsim_async_status", "amsim_debug_wait_report",
     "amsim_residual_norm", "amsim_residual_norm_grad_workspace", "amsim_residual_norm_grad",
-    "amsim_rotary",
+    "amsim_rotary", "amsim_adamw",
 ]
 
 
@@ -94,6 +94,8 @@ def _load() -> C.CDLL:
     L.amsim_residual_norm_grad_workspace.restype = sz
     L.amsim_residual_norm_grad.argtypes = [vp] * 17 + [ll, ip, ll, f, ip, ip, ip, vp, sz, u]
     L.amsim_rotary.argtypes = [vp, vp, vp, ip, vp, vp, ip, vp, vp, ll, ll, ip, ip, C.POINTER(ll), f, ip, u]
+    d = C.c_double
+    L.amsim_adamw.argtypes = [vp, ip] + [vp] * 9 + [d, vp, d, d, d, d, vp, u, ip, ip, ip]
     return L
 
 

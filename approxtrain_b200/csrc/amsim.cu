@@ -31,6 +31,7 @@
 #include "amsim_codes.cu"
 #include "amsim_norm.cu"
 #include "amsim_rotary.cu"
+#include "amsim_adamw.cu"
 #endif
 
 #include <atomic>

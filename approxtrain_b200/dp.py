@@ -67,13 +67,15 @@ class DataParallelSGD:
                 p.amsim_grad_sink = GradSink(p.grad, hook)
                 self._sinks.append(p.amsim_grad_sink)
 
+    _ALIGN = 1   # elements a gradient's place in its bucket is a multiple of
+
     def _close_bucket(self, params):
-        n = sum(p.numel() for p in params)
-        flat = torch.zeros(n, dtype=params[0].dtype, device=params[0].device)
+        room = [-(-p.numel() // self._ALIGN) * self._ALIGN for p in params]
+        flat = torch.zeros(sum(room), dtype=params[0].dtype, device=params[0].device)
         off = 0
-        for p in params:
+        for p, n in zip(params, room):
             p.grad = flat[off:off + p.numel()].view_as(p)
-            off += p.numel()
+            off += n
         self.buckets.append({"flat": flat, "params": params, "pending": len(params), "fired": {}, "launched": False})
 
     def _make_hook(self, bi):
@@ -207,3 +209,38 @@ class DataParallelSGD:
 
     def gradient_bytes(self) -> int:
         return sum(b["flat"].numel() * b["flat"].element_size() for b in self.buckets)
+
+
+class DataParallelAdamW(DataParallelSGD):
+    """The same trainer with AdamW (``ops.adamw_step``) as the replicated update: one launch over all parameters, moments in 32
+    bits or in 8 (``state_bits``), on CUDA devices.  The step count and the learning rate live on the device, so a captured step
+    (``capture``) counts on and follows ``set_lr`` when it is replayed.  Every rank rounds 8-bit moments with the same
+    `seed`: replicas stay identical.  Parameters of one axis (biases, norms) get no weight decay."""
+
+    _ALIGN = 4   # gradients on 16-byte boundaries
+
+    def __init__(self, model: torch.nn.Module, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32, seed: int = 0, bucket_bytes: int = 32 << 20, process_group=None):
+        from . import ops
+        super().__init__(model, lr, bucket_bytes=bucket_bytes, process_group=process_group)
+        self.betas, self.eps, self.seed = betas, eps, seed
+        self.decay = [weight_decay if p.dim() > 1 else 0.0 for p in self.params]
+        self.state = ops.AdamWState(self.params, bits=state_bits)
+        self._lr = torch.full((1,), lr, dtype=torch.float32, device=self.state.device)
+
+    def set_lr(self, lr: float) -> None:
+        self.lr = lr
+        self._lr.fill_(lr)
+
+    def _update(self):
+        from . import ops
+        with torch.no_grad():
+            ops.adamw_step(self.params, [p.grad for p in self.params], self.state, self._lr, betas=self.betas, eps=self.eps,
+                           weight_decay=self.decay, grad_scale=1.0 / self.world, seed=self.seed)
+
+    def state_dict(self) -> dict:
+        return {"lr": self.lr, "moments": self.state.state_dict()}
+
+    def load_state_dict(self, state: dict) -> None:
+        self.set_lr(state["lr"])
+        self.state.load_state_dict(state["moments"])

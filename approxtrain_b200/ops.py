@@ -31,12 +31,12 @@ import torch
 
 from . import _lib
 from ._lib import AmsimError, lib, check
-from .train_ops import residual_norm, residual_norm_grad, rotary, rotary_frequencies, RotaryFrequencies
+from .train_ops import AdamWState, RotaryFrequencies, adamw_step, residual_norm, residual_norm_grad, rotary, rotary_frequencies
 
 __all__ = [
     "AMLut", "get_lut", "am_multiply", "conv2d_geometry", "convam", "convam_input_grad", "convam_filter_grad",
     "denseam", "denseam_grad", "matmulam", "convam_bias_act", "denseam_bias_act", "bias_grad", "AmsimError",
-    "residual_norm", "residual_norm_grad", "rotary", "rotary_frequencies", "RotaryFrequencies",
+    "residual_norm", "residual_norm_grad", "rotary", "rotary_frequencies", "RotaryFrequencies", "adamw_step", "AdamWState",
 ]
 
 
@@ -455,7 +455,7 @@ def _install_nvtx_ranges() -> None:
         return
     g = globals()
     for name in ("am_multiply", "convam", "convam_bias_act", "denseam_bias_act", "convam_input_grad",
-                 "convam_filter_grad", "denseam", "denseam_grad", "matmulam", "bias_grad", "residual_norm", "residual_norm_grad", "rotary"):
+                 "convam_filter_grad", "denseam", "denseam_grad", "matmulam", "bias_grad", "residual_norm", "residual_norm_grad", "rotary", "adamw_step"):
         fn = g[name]
 
         def wrapped(*a, __fn=fn, __name=name, **k):

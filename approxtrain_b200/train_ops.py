@@ -3,6 +3,7 @@
 =====================  ==================================================================
 ``residual_norm``      norms before and after a block with its gate and residual scale
 ``rotary``             rotary positions of queries and keys
+``adamw_step``         one AdamW step over many tensors, moments in 32 bits or in 8
 =====================  ==================================================================
 
 Same manner as :mod:`approxtrain_b200.ops`, which exports all of them: torch CUDA tensors, one call into ``libamsim.so``
@@ -11,6 +12,7 @@ gradients.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 
@@ -296,3 +298,136 @@ def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half",
     _call(q.device, lib.amsim_rotary, q.data_ptr(), out.data_ptr(), q.shape[-2], _ptr(k_), _ptr(out2), k_.shape[-2] if k_ is not None else 0,
           positions.data_ptr(), freqs.inv_freq.data_ptr(), batch, seq, q.shape[-1], freqs.rotary_dim, strides, freqs.scale, _TYPES[q.dtype], flags)
     return out if k is None else (out, out2)
+
+
+# ---- AdamW ----------------------------------------------------------------------------------------
+ADAMW_BLOCK = 256     # elements that share a scale in 8-bit moments
+_contiguous, _numel, _device, _data_ptr = torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.data_ptr
+
+
+def _address(a: array.array):
+    return a.buffer_info()[0]
+
+
+class AdamWState:
+    """Moments and step count of ``adamw_step`` for a list of parameters (float32, bfloat16 or float16, all of one type, on one
+    device).
+
+    ``bits=32``: ``exp_avg`` and ``exp_avg_sq``, float32, parameter after parameter.  ``bits=8``: ``exp_avg`` and
+    ``exp_avg_sq_root`` (the square root of the second moment) as float8_e4m3fn, every parameter padded to a multiple of
+    256 elements, and the scale of every 256 (``exp_avg_scale``, ``exp_avg_sq_scale``): value = code * scale.
+    ``moments(i)`` gives those of parameter i in float32.  ``step``: int64 on the device, counted by the steps themselves."""
+
+    def __init__(self, params, bits: int = 32):
+        params = list(params)
+        if bits not in (8, 32):
+            raise ValueError(f"moments of 32 or 8 bits, got {bits}")
+        if not params:
+            raise ValueError("no parameters")
+        for i, p in enumerate(params):
+            _tensor(p, f"parameter {i}", params[0])
+            if p.dtype != params[0].dtype:
+                raise TypeError(f"parameters must have one type, got {p.dtype} beside {params[0].dtype}")
+        self.bits, self.device, self.dtype = bits, params[0].device, params[0].dtype
+        self.shapes = [tuple(p.shape) for p in params]
+        self.sizes = [p.numel() for p in params]
+        block = ADAMW_BLOCK if bits == 8 else 1
+        self._starts, at = [], 0
+        for n in self.sizes:
+            self._starts.append(at)
+            at += -(-n // block) * block
+        kw = dict(device=self.device)
+        if bits == 32:
+            self.exp_avg, self.exp_avg_sq = (torch.zeros(at, dtype=torch.float32, **kw) for _ in range(2))
+            self._moments = ("exp_avg", "exp_avg_sq")
+        else:
+            self.exp_avg, self.exp_avg_sq_root = (torch.zeros(at, dtype=torch.float8_e4m3fn, **kw) for _ in range(2))
+            self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(at // ADAMW_BLOCK, dtype=torch.float32, **kw) for _ in range(2))
+            self._moments = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_scale")
+        self._counter = torch.zeros(2, dtype=torch.int64, **kw)
+        self._sizes = array.array("q", self.sizes)
+
+    @property
+    def step(self) -> torch.Tensor:
+        return self._counter[0]
+
+    def moments(self, i: int):
+        """(exp_avg, exp_avg_sq) of parameter i in float32, in its shape."""
+        a, n = self._starts[i], self.sizes[i]
+        if self.bits == 32:
+            m, v = self.exp_avg[a:a + n], self.exp_avg_sq[a:a + n]
+        else:
+            b = slice(a // ADAMW_BLOCK, -(-(a + n) // ADAMW_BLOCK))
+            codes = slice(b.start * ADAMW_BLOCK, b.stop * ADAMW_BLOCK)
+            m = (self.exp_avg[codes].float().view(-1, ADAMW_BLOCK) * self.exp_avg_scale[b, None]).view(-1)[:n]
+            v = (self.exp_avg_sq_root[codes].float().view(-1, ADAMW_BLOCK) * self.exp_avg_sq_scale[b, None]).square().view(-1)[:n]
+        return m.view(self.shapes[i]), v.view(self.shapes[i])
+
+    def state_dict(self) -> dict:
+        return {"bits": self.bits, "shapes": list(self.shapes), "step": self.step.clone(), **{k: getattr(self, k).clone() for k in self._moments}}
+
+    def load_state_dict(self, state: dict) -> None:
+        if state["bits"] != self.bits or [tuple(s) for s in state["shapes"]] != self.shapes:
+            raise ValueError("the state is of other parameters or other bits")
+        with torch.no_grad():
+            self._counter[0] = state["step"].to(self.device)
+            for k in self._moments:
+                if state[k].shape != getattr(self, k).shape or state[k].dtype != getattr(self, k).dtype:
+                    raise ValueError(f"{k} does not match")
+            for k in self._moments:
+                getattr(self, k).copy_(state[k])
+
+
+def _rate(value, name, device):
+    """(number, address of a number on the device)."""
+    if not isinstance(value, torch.Tensor):
+        return float(value), None
+    if value.dtype != torch.float32 or value.numel() != 1 or value.device != device:
+        raise ValueError(f"{name} must be a number or a float32 tensor of one element on {device}")
+    return 1.0, value.data_ptr()
+
+
+def adamw_step(params, grads, state: AdamWState, lr, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.0, grad_scale=1.0, seed: int = 0) -> None:
+    """One AdamW step (weight decay beside the gradient) over `params`, in place, with the moments and the step count in
+    `state`; in FP32 whatever the types, two launches at most up to 1280 tensors.
+
+    ``p -= lr * weight_decay * p``; ``m = b1 m + (1 - b1) g``; ``v = b2 v + (1 - b2) g^2``;
+    ``p -= lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)``, g = grad * grad_scale.
+
+    `params`, `grads`: lists in the order of the state, dense, of any alignment; gradients have the parameters' type or
+    are float32.  `weight_decay`: a number, or one per parameter.  `lr`, `grad_scale`: numbers, or float32 tensors of
+    one element on the device (read when the step runs, so a captured step follows them).  `seed`: of the random rounding
+    of 8-bit moments.  Gradients have to be finite: one that is not makes its block's moments and its parameter so."""
+    if not isinstance(state, AdamWState):
+        raise TypeError("state must be an AdamWState")
+    n = len(state.sizes)
+    for ts, name in ((params, "params"), (grads, "grads")):
+        if len(ts) != n:
+            raise ValueError(f"{n} {name} expected, got {len(ts)}")
+        if list(map(_numel, ts)) != state.sizes:
+            raise ValueError(f"the sizes of {name} are not those of the state's parameters")
+        if not all(map(_contiguous, ts)):
+            raise ValueError(f"{name} must be contiguous")
+        if set(map(_device, ts)) != {state.device.index}:
+            raise ValueError(f"{name} must be on {state.device}")
+    types = {t.dtype for t in grads}
+    if {t.dtype for t in params} != {state.dtype} or len(types) != 1 or not types <= {state.dtype, torch.float32}:
+        raise TypeError(f"params must be {state.dtype}, grads all {state.dtype} or all float32")
+    if isinstance(weight_decay, (int, float)):
+        decay = array.array("f", (weight_decay,)) * n
+    else:
+        decay = array.array("f", weight_decay)
+        if len(decay) != n:
+            raise ValueError(f"weight_decay: a number or {n} of them, got {len(decay)}")
+    b1, b2 = betas
+    if not (0 <= b1 < 1 and 0 <= b2 < 1) or not eps >= 0:
+        raise ValueError(f"betas in [0, 1) and eps >= 0 expected, got {betas}, {eps}")
+    lr, lr_at = _rate(lr, "lr", state.device)
+    scale, scale_at = _rate(grad_scale, "grad_scale", state.device)
+    p_at, g_at = array.array("Q", map(_data_ptr, params)), array.array("Q", map(_data_ptr, grads))
+    if state.bits == 32:
+        m, ms, v, vs = state.exp_avg.data_ptr(), None, state.exp_avg_sq.data_ptr(), None
+    else:
+        m, ms, v, vs = (getattr(state, k).data_ptr() for k in state._moments)
+    _call(state.device, lib.amsim_adamw, n, _address(p_at), _address(g_at), _address(state._sizes), _address(decay), m, ms, v, vs,
+          state._counter.data_ptr(), lr, lr_at, b1, b2, eps, scale, scale_at, seed & 0xFFFFFFFF, _TYPES[state.dtype], _TYPES[types.pop()], state.bits)

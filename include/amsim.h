@@ -341,6 +341,23 @@ int amsim_rotary(void* stream, const void* x, void* out, int heads, const void* 
                  long long seq, int dim, int rotary_dim, const long long* strides, float scale,
                  int dtype, unsigned flags);
 
+/* ---- AdamW -----------------------------------------------------------------------------
+ * (No reference counterpart: its scripts call Keras optimizers.)
+ * One step over `tensors` parameters (dense, any alignment; sizes in elements; sizes and the arrays of pointers are host memory,
+ * read before the call returns): p -= lr * decay[i] * p, the moments, p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),
+ * all in FP32.  Parameters have `dtype`, gradients (times grad_scale) dtype or AMSIM_F32.  `step` (device, two int64, the
+ * second zero): steps taken, one more after the call.  lr_dev and grad_scale_dev (device, may be NULL): lr instead of
+ * `lr`, and a further factor of the gradients, read when the kernel runs.
+ * bits 32: exp_avg and exp_avg_sq are FP32, tensor after tensor.  bits 8: E4M3 codes of m and of sqrt(v), every tensor padded to a
+ * multiple of 256, with one FP32 scale per 256 (code value * scale; 448 * scale is the block's largest); rounded up or down
+ * at random, in proportion, from `seed`, the step and the place.  Moments are 16-byte aligned and zero before the first
+ * step.  Gradients have to be finite. */
+int amsim_adamw(void* stream, int tensors, const void* const* params, const void* const* grads,
+                const long long* sizes, const float* decay, void* exp_avg, float* exp_avg_scale,
+                void* exp_avg_sq, float* exp_avg_sq_scale, long long* step, double lr,
+                const float* lr_dev, double beta1, double beta2, double eps, double grad_scale,
+                const float* grad_scale_dev, unsigned seed, int dtype, int grad_dtype, int bits);
+
 /* Number of kernels this library has launched since it was loaded (all devices, all
  * streams).  For benchmarks that report their launch count; no reference counterpart. */
 unsigned long long amsim_debug_launch_count(void);

@@ -117,3 +117,32 @@ def test_rotary_refusals(L):
     other = (C.c_longlong * 14)(64, 16, 8, 64, 16, 4, 0, 0, 0, 0, 0, 0, 0, 1)
     assert call(out=p, st=other) == L.ERR_INVALID and b"in place" in L.lib.amsim_last_error()
     assert call(batch=0) == 0 and call(heads=0) == 0
+
+
+def test_adamw_abi_refusals(L):
+    import array
+    p = 1 << 20
+    one = array.array("Q", [p, p])
+    n = array.array("q", [8, 3])
+    dec = array.array("f", [0.0, 0.0])
+    at = lambda a: a.buffer_info()[0]
+
+    def call(tensors=2, params=at(one), grads=at(one), sizes=at(n), decay=at(dec), m=p, ms=None, v=p, vs=None, step=p, b1=0.9, b2=0.99, eps=1e-8,
+             types=(0, 0), bits=32):
+        return L.lib.amsim_adamw(None, tensors, params, grads, sizes, decay, m, ms, v, vs, step, 0.1, None, b1, b2, eps, 1.0, None, 0, *types, bits)
+    assert call(tensors=-1) == L.ERR_INVALID
+    assert call(bits=16) == L.ERR_INVALID
+    assert call(types=(3, 0)) == L.ERR_INVALID and call(types=(1, 2)) == L.ERR_INVALID and call(types=(0, 1)) == L.ERR_INVALID
+    assert call(b1=1.0) == L.ERR_INVALID and call(b2=-0.1) == L.ERR_INVALID and call(eps=float("nan")) == L.ERR_INVALID
+    assert call(step=None) == L.ERR_INVALID and call(params=None) == L.ERR_INVALID and call(decay=None) == L.ERR_INVALID
+    assert call(m=None) == L.ERR_INVALID and call(m=p + 4) == L.ERR_INVALID and call(bits=8) == L.ERR_INVALID
+    bad = array.array("q", [8, -1])
+    assert call(sizes=at(bad)) == L.ERR_INVALID
+    null = array.array("Q", [p, 0])
+    assert call(grads=at(null)) == L.ERR_INVALID
+
+
+def test_adamw_refuses_cpu_tensors(L):
+    from approxtrain_b200 import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.AdamWState([torch.zeros(3)])
