@@ -32,6 +32,7 @@
 #include "amsim_norm.cu"
 #include "amsim_rotary.cu"
 #include "amsim_adamw.cu"
+#include "amsim_mx.cu"
 #endif
 
 #include <atomic>
@@ -213,7 +214,12 @@ int stuck_words_open() {
   std::lock_guard<std::mutex> lk(mu);
   if (g_stuck.load()) return AMSIM_OK;
   void* p = nullptr;
-  CUDA_TRY(cudaHostAlloc(&p, kMostDevices * sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped));
+  // (host memory, nothing that a capture of this thread records: allowed while one is under way)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+  const cudaError_t got = cudaHostAlloc(&p, kMostDevices * sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped);
+  CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+  CUDA_TRY(got);
   memset(p, 0, kMostDevices * sizeof(unsigned));
   g_stuck.store(static_cast<unsigned*>(p));
   return AMSIM_OK;
@@ -243,6 +249,13 @@ int host_fail(int code, const char* fmt, ...) {
 void host_count_launch() { AMSIM_COUNT_LAUNCH(); }
 int host_sm_count(int device) { return sm_count(device); }
 int host_device() { return current_device(); }
+int host_stuck_word(int device, unsigned** word) {
+  if (device < 0 || device >= kMostDevices) return fail(AMSIM_ERR_UNSUPPORTED, "device %d of at most %d", device, kMostDevices);
+  if (const int rc = stuck_words_open()) return rc;
+  *word = g_stuck.load() + device;
+  return AMSIM_OK;
+}
+int host_report_stuck(int device) { return report_stuck(device); }
 
 }  // namespace amsim
 

@@ -11,6 +11,10 @@ int host_fail(int code, const char* fmt, ...);  // records the text, returns cod
 void host_count_launch();
 int host_sm_count(int device);
 int host_device();
+// A word in host memory that a kernel on `device` sets when a bounded wait of its warps has run out; reported, once, as
+// AMSIM_ERR_CUDA by the next call that asks.
+int host_stuck_word(int device, unsigned** word);
+int host_report_stuck(int device);
 
 }  // namespace amsim
 

@@ -474,3 +474,78 @@ def rotary(q, positions, freqs, k=None, layout="half"):
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, positions, freqs, layout)
     return ops.rotary(q, positions, freqs, k=k, layout=layout)
+
+
+class _MXDenseFn(torch.autograd.Function):
+    """A dense layer whose three products are taken in 4-bit floats.  Every operand is quantised along the axis that its
+    product contracts: x and w along both (one read), and so is the gradient.  What is kept for the backward pass is
+    the 4-bit copies, not x and w."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, activation):
+        want_x, want_w = ctx.needs_input_grad[:2]
+        x_rows, x_cols = ops.mx_quantize_both(x) if want_w else (ops.mx_quantize(x), None)
+        w_rows, w_cols = ops.mx_quantize_both(w) if want_x else (None, ops.mx_quantize(w, axis=0))
+        y = ops.mx_matmul(x_rows, w_cols, bias=bias, activation=activation, out_dtype=x.dtype)
+        ctx.save_for_backward(x_cols.data if want_w else None, w_rows.data if want_x else None, y if activation == "relu" else None)
+        ctx.cfg = (tuple(x.shape), tuple(w.shape), x.dtype, w.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x_data, w_data, y = ctx.saved_tensors
+        x_shape, w_shape, x_type, w_type = ctx.cfg
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        g = (torch.ops.aten.threshold_backward(g, y, 0.0) if y is not None else g).contiguous()
+        if want_x and want_w:
+            g_rows, g_cols = ops.mx_quantize_both(g)
+        else:
+            g_rows, g_cols = (ops.mx_quantize(g) if want_x else None), (ops.mx_quantize(g, axis=0) if want_w else None)
+        dx = ops.mx_matmul(g_rows, ops.MXTensor(w_data, w_shape, 1), out_dtype=x_type) if want_x else None
+        dw = ops.mx_matmul(ops.MXTensor(x_data, x_shape, 0), g_cols, out_dtype=w_type) if want_w else None
+        db = None
+        if want_b:
+            db = ops.bias_grad(g) if g.dtype == torch.float32 else g.sum(0, dtype=torch.float32)
+        return dx, dw, db, None
+
+
+def mxdense(x, w, bias=None, activation=None):
+    """``act(x w + bias)`` on the last axis with the products in 4-bit floats (``ops.mx_matmul``), forward and backward; x [..., in],
+    w [in, out], float32, bfloat16 or float16; bias float32.  ``activation``: None or "relu"."""
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[0]:
+        raise ValueError(f"x [..., in] and w [in, out] expected, got {list(x.shape)} and {list(w.shape)}")
+    lead = x.shape[:-1]
+    y = _MXDenseFn.apply(x.reshape(-1, x.shape[-1]), w, bias, activation)
+    return y.reshape(*lead, w.shape[1])
+
+
+class densemx(nn.Module):
+    """Dense layer in 4-bit floats: the counterpart of ``denseam`` with the hardware's block-scaled products instead of a
+    multiplier's table.  ``freeze()`` keeps the weights quantised for inference."""
+
+    def __init__(self, in_features, units, activation=None, use_bias=True, kernel_initializer="glorot_uniform"):
+        super().__init__()
+        template = denseam(in_features, units, activation=activation, use_bias=use_bias, kernel_initializer=kernel_initializer)
+        self.activation = activation
+        self.kernel, self.bias = template.kernel, template.bias
+        self._frozen = None
+
+    def freeze(self):
+        """Quantises the weights once; later calls use them until ``train()`` is called."""
+        self._frozen = ops.mx_quantize(self.kernel.detach(), axis=0)
+        return self.eval()
+
+    def train(self, mode=True):
+        if mode:
+            self._frozen = None
+        return super().train(mode)
+
+    def forward(self, x):
+        fused = self.activation if self.activation in (None, "linear", "relu") else None
+        if self._frozen is not None:
+            y = ops.mx_matmul(ops.mx_quantize(x.reshape(-1, x.shape[-1])), self._frozen, bias=self.bias, activation=fused, out_dtype=x.dtype)
+            y = y.reshape(*x.shape[:-1], self.kernel.shape[1])
+        else:
+            y = mxdense(x, self.kernel, self.bias, fused)
+        return y if fused == self.activation else _ACT[self.activation](y)

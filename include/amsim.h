@@ -358,6 +358,26 @@ int amsim_adamw(void* stream, int tensors, const void* const* params, const void
                 const float* lr_dev, double beta1, double beta2, double eps, double grad_scale,
                 const float* grad_scale_dev, unsigned seed, int dtype, int grad_dtype, int bits);
 
+/* ---- 4-bit products -----------------------------------------------------------------------
+ * (No reference counterpart: block-scaled 4-bit floats as the hardware multiplies them, beside the tables that simulate a
+ * multiplier.)  Matrices in the OCP microscaling format MXFP4: E2M1 elements, an E8M0 scale for each 32 along the axis that a product
+ * contracts, in the library's own tiles (amsim_mx_bytes(rows, k): a matrix of `rows` rows whose axis of length k is
+ * quantised, 16-byte aligned).
+ *
+ * Quantise: x (rows x cols, dense) along its columns' axis into `along` (rows x cols) and / or along its rows' axis into
+ * `across` (cols x rows, k = rows); either may be NULL, both take one read of x.  Scale of a block: the power of two that puts its
+ * largest element in [4, 8); elements are rounded to nearest, ties to even, beyond 6 to 6.  An infinity or NaN makes its
+ * block NaN.  Dequantise: `transposed` writes k x rows (a matrix quantised across, as it was). */
+size_t amsim_mx_bytes(long long rows, long long k);
+int amsim_mx_quantize(void* stream, const void* x, long long rows, long long cols, int dtype,
+                      void* along, void* across);
+int amsim_mx_dequantize(void* stream, const void* data, long long rows, long long k,
+                        int transposed, void* out, int dtype);
+/* out[i][j] = act(sum over k of a[i][k] b[j][k] + bias[j]), out m x n dense of `dtype`; bias (n floats) may be NULL.  Products are
+ * exact, sums FP32 (within 2e-6 of the exact ones' norm for FP32 outputs). */
+int amsim_mx_matmul(void* stream, const void* a, const void* b, long long m, long long n,
+                    long long k, const float* bias, int act, void* out, int dtype);
+
 /* Number of kernels this library has launched since it was loaded (all devices, all
  * streams).  For benchmarks that report their launch count; no reference counterpart. */
 unsigned long long amsim_debug_launch_count(void);

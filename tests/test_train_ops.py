@@ -146,3 +146,23 @@ def test_adamw_refuses_cpu_tensors(L):
     from approxtrain_b200 import ops
     with pytest.raises(ValueError, match="CUDA"):
         ops.AdamWState([torch.zeros(3)])
+
+
+def test_mx_refusals(L):
+    from approxtrain_b200 import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.mx_quantize(torch.zeros(2, 4))
+    p = 1 << 20
+    q, d, m = L.lib.amsim_mx_quantize, L.lib.amsim_mx_dequantize, L.lib.amsim_mx_matmul
+    assert L.lib.amsim_mx_bytes(1, 1) == 17408 and L.lib.amsim_mx_bytes(129, 257) == 4 * 17408 and L.lib.amsim_mx_bytes(0, 5) == 0 and L.lib.amsim_mx_bytes(5, 0) == 17408
+    assert q(None, p, -1, 4, 0, p, None) == L.ERR_INVALID and q(None, p, 4, 4, 3, p, None) == L.ERR_INVALID
+    assert q(None, p, 4, 4, 0, None, None) == L.ERR_INVALID and q(None, None, 4, 4, 0, p, None) == L.ERR_INVALID
+    assert q(None, p, 4, 4, 0, p + 8, None) == L.ERR_INVALID and q(None, p, 1 << 31, 4, 0, p, None) == L.ERR_UNSUPPORTED
+    assert q(None, p, 1 << 21, 1 << 21, 0, p, None) == L.ERR_UNSUPPORTED
+    assert q(None, None, 0, 4, 0, p, None) == 0
+    assert d(None, p, 4, -1, 0, p, 0) == L.ERR_INVALID and d(None, None, 4, 4, 0, p, 0) == L.ERR_INVALID and d(None, p + 4, 4, 4, 0, p, 0) == L.ERR_INVALID
+    assert d(None, p, 4, 4, 0, p, 5) == L.ERR_INVALID and d(None, None, 0, 4, 0, None, 0) == 0
+    assert m(None, p, p, -1, 4, 4, None, 0, p, 0) == L.ERR_INVALID and m(None, p, p, 4, 4, 4, None, 2, p, 0) == L.ERR_INVALID
+    assert m(None, p, p, 4, 4, 4, None, 0, p, 3) == L.ERR_INVALID and m(None, None, p, 4, 4, 4, None, 0, p, 0) == L.ERR_INVALID
+    assert m(None, p + 8, p, 4, 4, 4, None, 0, p, 0) == L.ERR_INVALID and m(None, p, p, 1 << 30, 1 << 30, 4, None, 0, p, 0) == L.ERR_UNSUPPORTED
+    assert m(None, p, p, 0, 4, 4, None, 0, p, 0) == 0
