@@ -24,31 +24,36 @@ namespace amsim {
 namespace normk {
 
 constexpr int MAX_THREADS = 512;
+constexpr int SHARED_CTA = 256;   // threads of a CTA that several rows share
+constexpr int GROUPS = 4;         // rows of more than a warp each that may share a CTA
 
 struct NormParams {
   const void *x, *block, *gate, *post_w, *post_b, *pre_w, *pre_b;
   void *sum, *y;
   float* stats;              // rows x 4: mean and 1 / deviation of N_post, then of N_pre
   const void *dsum, *dy;     // backward
-  int n_in;                  // tensors fetched ahead, and the places of x, block, dy, dsum among them
-  int in_x, in_block, in_dy, in_dsum;
+  int n_in;                  // tensors fetched ahead, and the places of x, block, dy, dsum and a gate of one row per row among them
+  int in_x, in_block, in_dy, in_dsum, in_gate;
   void *dx, *dblock, *dgate, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
-  float *part, *gate_part;   // column sums: [workers][arrays][width], [workers][2][width]
+  float *part, *gate_part;   // column sums: [teams][4][width], [workers][2][width]
   long long rows, per_gate;  // rows that share a row of the gate
-  long long per_worker;      // rows of a worker (backward)
+  long long per_worker;      // consecutive rows of a worker (the threads of one row)
   long long workers;
   int width, tpr, tpr_log, cluster;
   int w_type, gate_type;
   float scale, eps, inv_width;
-  int post, pre;
+  int pre;
 };
+
+// What a gate is to the kernels: none; rows shared by several rows, kept like the weights; or one row for each row, fetched ahead.
+constexpr int GATE_NONE = 0, GATE_SHARED = 1, GATE_ROWS = 2;
 
 // Sums over the threads of a row.  Two buffers per sum: a warp that runs ahead writes the other one, and cannot come back to
 // the first before everybody has passed the barrier between.
 struct RowSum {
-  float* red;     // [2][2][16] partial sums of the CTA's warps
+  float* red;     // [2][2][16] partial sums of the row's warps
   float* peers;   // [2][2][8] partial sums of the cluster's CTAs
-  int tpr, cluster, rank, buf;
+  int tpr, cluster, rank, group, buf;
 
   __device__ __forceinline__ void operator()(float& a, float& b, bool both) {
     const int lanes = tpr < 32 ? tpr : 32;
@@ -57,17 +62,18 @@ struct RowSum {
       if (both) b += __shfl_xor_sync(0xffffffffu, b, o);
     }
     if (tpr <= 32) return;
-    const int w = threadIdx.x >> 5;
+    const int warps = tpr >> 5, w = (threadIdx.x >> 5) & (warps - 1);
     if ((threadIdx.x & 31) == 0) {
       red[buf * 32 + w] = a;
       if (both) red[buf * 32 + 16 + w] = b;
     }
-    __syncthreads();
-    a = 0.f;
-    b = 0.f;
-    for (int i = 0; i < (tpr >> 5); ++i) {
-      a += red[buf * 32 + i];
-      if (both) b += red[buf * 32 + 16 + i];
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(tpr) : "memory");  // (the row's threads)
+    const int from = buf * 32 + (threadIdx.x & (warps - 1));
+    a = red[from];
+    if (both) b = red[from + 16];
+    for (int o = warps >> 1; o; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (both) b += __shfl_xor_sync(0xffffffffu, b, o);
     }
     if (cluster > 1) {
       if (threadIdx.x < cluster) {
@@ -87,17 +93,17 @@ struct RowSum {
   }
 };
 
-// Where a thread's elements are: chunk c holds columns at(c) .. at(c) + V - 1.
-template <int V>
+// Where a thread's elements are: chunk c holds columns at(c) .. at(c) + V - 1.  FULL: every chunk of every thread exists.
+template <int V, bool FULL>
 struct Cols {
   int first, step, width;
   __device__ __forceinline__ int at(int c) const { return first + c * step; }
-  __device__ __forceinline__ bool ok(int c) const { return at(c) < width; }
+  __device__ __forceinline__ bool ok(int c) const { return FULL || at(c) < width; }
 };
 
 // Rows fetched ahead of their use, each thread its own 16-byte chunks: stage, tensor, chunk.  Without 16-byte chunks (V = 1) elements are
 // loaded when they are needed.
-template <typename T, int V, int N>
+template <typename T, int V, int N, bool FULL>
 struct Ahead {
   static constexpr int STAGES = sizeof(T) == 4 ? 2 : 3;
   uint32_t base;
@@ -106,14 +112,17 @@ struct Ahead {
     base = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
   }
   __device__ __forceinline__ uint32_t place(int st, int k, int c) const { return base + ((st * n_in + k) * N + c) * (blockDim.x * 16); }
-  // tensor number k of row `at` into the stage that is `ahead` uses away
-  __device__ __forceinline__ void fetch(int ahead, int k, const void* src, long long at, bool live, const Cols<V>& cols) const {
-    if (V == 1 || !src || !live) return;
-    const int st = stage + ahead >= STAGES ? stage + ahead - STAGES : stage + ahead;
+  // tensor number k of the row whose first element of this thread is number `at`, into stage `st`
+  __device__ __forceinline__ void fetch(int st, int k, const void* src, long long at, const Cols<V, FULL>& cols) const {
+    if (V == 1 || !src) return;
+    const T* from = static_cast<const T*>(src) + at;
+    uint32_t to = place(st, k, 0);
 #pragma unroll
-    for (int c = 0; c < N; ++c)
-      if (cols.ok(c))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(st, k, c)), "l"(static_cast<const T*>(src) + at + cols.at(c)) : "memory");
+    for (int c = 0; c < N; ++c) {
+      if (cols.ok(c)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+      from += cols.step;
+      to += blockDim.x * 16;
+    }
   }
   __device__ __forceinline__ void commit() const {
     if (V > 1) asm volatile("cp.async.commit_group;" ::: "memory");
@@ -121,8 +130,10 @@ struct Ahead {
   __device__ __forceinline__ void ready() const {
     if (V > 1) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
   }
+  // the stage that is filled while `stage` is used: the one used before it
+  __device__ __forceinline__ int free_stage() const { return stage == 0 ? STAGES - 1 : stage - 1; }
   __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
-  __device__ __forceinline__ void read(int k, int c, const void* src, long long at, const Cols<V>& cols, float (&o)[V]) const {
+  __device__ __forceinline__ void read(int k, int c, const void* src, long long at, const Cols<V, FULL>& cols, float (&o)[V]) const {
     if constexpr (V == 1) {
       load_vec<T, 1>(src, at + cols.at(c), o);
     } else {
@@ -133,8 +144,63 @@ struct Ahead {
   }
 };
 
-template <bool LAYER, int N, int V>
-__device__ __forceinline__ void row_stats(const float (&z)[N][V], const Cols<V>& cols, const NormParams& p, RowSum& sum, float& mean, float& rstd) {
+// Weights, biases and the gate's row of a thread's columns, as FP32 in places of its own in shared memory: read for every row
+// without a look at their type or at whether they exist.
+template <int V, int N, bool FULL>
+struct Kept {
+  float* base;
+  __device__ __forceinline__ Kept(void* smem) : base(static_cast<float*>(smem) + threadIdx.x * (V == 1 ? 1 : 4)) {}
+  __device__ __forceinline__ float* place(int a, int c, int f) const {
+    return V == 1 ? base + (a * N + c) * (int)blockDim.x : base + ((a * N + c) * (V / 4) + f) * (4 * (int)blockDim.x);
+  }
+  __device__ __forceinline__ void keep(int a, const void* src, long long at, bool f32, int t16, float absent, const Cols<V, FULL>& cols) const {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = absent;
+      if (src && cols.ok(c)) load_param<V>(src, at + cols.at(c), f32, t16, v);
+      if constexpr (V == 1) {
+        *place(a, c, 0) = v[0];
+      } else {
+#pragma unroll
+        for (int f = 0; f < V / 4; ++f) *reinterpret_cast<float4*>(place(a, c, f)) = make_float4(v[4 * f], v[4 * f + 1], v[4 * f + 2], v[4 * f + 3]);
+      }
+    }
+  }
+  __device__ __forceinline__ void read(int a, int c, float (&o)[V]) const {
+    if constexpr (V == 1) {
+      o[0] = *place(a, c, 0);
+    } else {
+#pragma unroll
+      for (int f = 0; f < V / 4; ++f) {
+        const float4 v = *reinterpret_cast<const float4*>(place(a, c, f));
+        o[4 * f] = v.x; o[4 * f + 1] = v.y; o[4 * f + 2] = v.z; o[4 * f + 3] = v.w;
+      }
+    }
+  }
+};
+
+// Places among the kept arrays: N_pre's weight and bias (forward), N_post's, the gate.
+template <bool LAYER, bool POST, int GATE, bool BWD>
+struct Places {
+  static constexpr int PRE_W = 0, PRE_B = 1, POST_W = LAYER && !BWD ? 2 : 1, POST_B = POST_W + 1, GATE_V = POST_W + (POST ? LAYER ? 2 : 1 : 0);
+  static constexpr int COUNT = GATE_V + (GATE == GATE_SHARED ? 1 : 0);
+};
+
+// Elements per thread: as many of 16 and 8 as keep a thread's share of shared memory (512 threads a multiprocessor) and, backward,
+// its column sums in registers.
+template <typename T, bool LAYER, bool POST, int GATE>
+__host__ __device__ constexpr int fwd_elems() {
+  return 16 * 4 * Places<LAYER, POST, GATE, false>::COUNT + (sizeof(T) == 4 ? 2 * 64 : 3 * 32) * (GATE == GATE_ROWS ? 3 : 2) <= 440 ? 16 : 8;
+}
+template <typename T, bool LAYER, bool POST, int GATE>
+__host__ __device__ constexpr int bwd_elems() {
+  return POST || GATE != GATE_NONE || sizeof(T) == 4 ? 8 : 16;
+}
+
+template <bool LAYER, int N, int V, bool FULL>
+__device__ __forceinline__ void row_stats(const float (&z)[N][V], const Cols<V, FULL>& cols, const NormParams& p, RowSum& sum, float& mean, float& rstd) {
   float s = 0.f, none = 0.f;
   mean = 0.f;
   if (LAYER) {
@@ -148,109 +214,153 @@ __device__ __forceinline__ void row_stats(const float (&z)[N][V], const Cols<V>&
   s = 0.f;
 #pragma unroll
   for (int c = 0; c < N; ++c)
-    if (cols.ok(c)) {
+    if (!LAYER || cols.ok(c)) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += (z[c][e] - mean) * (z[c][e] - mean);
+      for (int e = 0; e < V; ++e) {
+        const float d = LAYER ? z[c][e] - mean : z[c][e];
+        s += d * d;
+      }
     }
   sum(s, none, false);
   rstd = 1.f / sqrtf(s * p.inv_width + p.eps);
 }
 
-template <bool LAYER, int N, int V>
-__device__ __forceinline__ void affine(float (&z)[N][V], const Cols<V>& cols, const void* w, const void* b, int type16, bool f32, float mean, float rstd) {
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    if (!cols.ok(c)) continue;
-    float wv[V], bv[V];
-    if (w) load_param<V>(w, cols.at(c), f32, type16, wv);
-    if (LAYER && b) load_param<V>(b, cols.at(c), f32, type16, bv);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float h = LAYER ? (z[c][e] - mean) * rstd : z[c][e] * rstd;
-      if (w) h *= wv[e];
-      if (LAYER && b) h += bv[e];
-      z[c][e] = h;
-    }
+// The rows of a worker and the gate's row that they share, walked in order.
+struct Walk {
+  long long row, last, at, gate_row, gate_left;  // at: first element; gate_left: rows until the gate's next one
+  __device__ __forceinline__ Walk(const NormParams& p, long long worker) {
+    row = min(worker * p.per_worker, p.rows);
+    last = min(row + p.per_worker, p.rows);
+    at = row * p.width;
+    gate_row = row / p.per_gate;
+    gate_left = p.per_gate - (row - gate_row * p.per_gate);
   }
-}
+  __device__ __forceinline__ bool live() const { return row < last; }
+  // true where the gate's next row begins
+  __device__ __forceinline__ bool next(const NormParams& p) {
+    ++row;
+    at += p.width;
+    if (--gate_left) return false;
+    gate_left = p.per_gate;
+    ++gate_row;
+    return true;
+  }
+};
 
-template <typename T, int V, bool LAYER, int E>
+template <typename T, int V, bool LAYER, bool POST, int GATE, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_fwd(const __grid_constant__ NormParams p) {
-  constexpr int N = E / V;
-  __shared__ float red[64], peers[32];
+  constexpr int N = fwd_elems<T, LAYER, POST, GATE>() / V;
+  using A = Ahead<T, V, N, FULL>;
+  using P = Places<LAYER, POST, GATE, false>;
+  __shared__ float red[GROUPS][64], peers[32];
   extern __shared__ __align__(16) uint8_t smem[];
   const int t = threadIdx.x & (p.tpr - 1), group = threadIdx.x >> p.tpr_log, groups = blockDim.x >> p.tpr_log;
   const int rank = blockIdx.x % p.cluster;
-  RowSum sum{red, peers, p.tpr, p.cluster, rank, 0};
-  const Cols<V> cols{(rank * N * p.tpr + t) * V, p.tpr * V, p.width};
-  const long long step = (long long)(gridDim.x / p.cluster) * groups;
-  Ahead<T, V, N> in(p, smem);
-  constexpr int STAGES = Ahead<T, V, N>::STAGES;
-  auto fetch = [&](int ahead, long long row) {
-    in.fetch(ahead, p.in_x, p.x, row * p.width, row < p.rows, cols);
-    in.fetch(ahead, p.in_block, p.block, row * p.width, row < p.rows, cols);
+  RowSum sum{red[group & (GROUPS - 1)], peers, p.tpr, p.cluster, rank, group, 0};
+  const Cols<V, FULL> cols{(rank * N * p.tpr + t) * V, p.tpr * V, p.width};
+  Walk w(p, (long long)(blockIdx.x / p.cluster) * groups + group);
+  A in(p, smem);
+  const Kept<V, N, FULL> kept(smem + (V == 1 ? 0 : A::STAGES * p.n_in * N * 16 * (int)blockDim.x));
+  long long to_fetch = w.last - w.row, fetch_at = w.at + cols.first;
+  auto fetch = [&](int st) {
+    if (to_fetch > 0) {
+      in.fetch(st, p.in_x, p.x, fetch_at, cols);
+      in.fetch(st, p.in_block, p.block, fetch_at, cols);
+      if (GATE == GATE_ROWS) in.fetch(st, p.in_gate, p.gate, fetch_at, cols);
+      fetch_at += p.width;
+      --to_fetch;
+    }
     in.commit();
   };
-  const long long begin = (long long)(blockIdx.x / p.cluster) * groups;
-  for (int i = 0; i < STAGES - 1; ++i) fetch(i, begin + group + i * step);
-  for (long long base = begin; base < p.rows; base += step, in.next()) {  // (the same trips for all threads)
-    const long long row = base + group;
-    const bool live = row < p.rows;
-    const long long at = row * p.width;
+  for (int i = 0; i < A::STAGES - 1; ++i) fetch(i);
+  const bool w32 = p.w_type == 0, g32 = p.gate_type == 0;
+  if (p.pre) {
+    kept.keep(P::PRE_W, p.pre_w, 0, w32, type16<T>(), 1.f, cols);
+    if (LAYER) kept.keep(P::PRE_B, p.pre_b, 0, w32, type16<T>(), 0.f, cols);
+  }
+  if (POST) {
+    kept.keep(P::POST_W, p.post_w, 0, w32, type16<T>(), 1.f, cols);
+    if (LAYER) kept.keep(P::POST_B, p.post_b, 0, w32, type16<T>(), 0.f, cols);
+  }
+  bool new_gate = true;
+  for (long long i = 0; i < p.per_worker; ++i, in.next()) {  // (the same trips for all threads)
+    const bool live = w.live();
     float r[N][V], u[N][V];
-    fetch(STAGES - 1, row + (STAGES - 1) * step);
+    fetch(in.free_stage());
+    if (GATE == GATE_SHARED && live && new_gate) kept.keep(P::GATE_V, p.gate, w.gate_row * p.width, g32, type16<T>(), 0.f, cols);
     in.ready();
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) r[c][e] = u[c][e] = 0.f;
       if (live && cols.ok(c)) {
-        in.read(p.in_x, c, p.x, at, cols, r[c]);
-        if (p.block) in.read(p.in_block, c, p.block, at, cols, u[c]);
+        in.read(p.in_x, c, p.x, w.at, cols, r[c]);
+        if (p.block) in.read(p.in_block, c, p.block, w.at, cols, u[c]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[c][e] = u[c][e] = 0.f;
       }
     }
-    if (p.block) {
-      if (p.post) {
-        float mean, rstd;
-        row_stats<LAYER>(u, cols, p, sum, mean, rstd);
-        affine<LAYER>(u, cols, p.post_w, p.post_b, type16<T>(), p.w_type == 0, mean, rstd);
-        if (p.stats && live && t == 0 && rank == 0) *reinterpret_cast<float2*>(p.stats + row * 4) = make_float2(mean, rstd);
-      }
-      const long long gate_at = p.gate && live ? row / p.per_gate * p.width : 0;
+    if (POST) {
+      float mean, rstd;
+      row_stats<LAYER>(u, cols, p, sum, mean, rstd);
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        if (!live || !cols.ok(c)) continue;
-        float gv[V];
-        if (p.gate) load_param<V>(p.gate, gate_at + cols.at(c), p.gate_type == 0, type16<T>(), gv);
+        float wv[V], bv[V];
+        kept.read(P::POST_W, c, wv);
+        if (LAYER) kept.read(P::POST_B, c, bv);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float b = p.gate ? u[c][e] * gv[e] : u[c][e];
-          r[c][e] += p.scale * b;
+        for (int e = 0; e < V; ++e) u[c][e] = LAYER ? (u[c][e] - mean) * rstd * wv[e] + bv[e] : u[c][e] * rstd * wv[e];
+      }
+      if (p.stats && live && t == 0 && rank == 0) *reinterpret_cast<float2*>(p.stats + w.row * 4) = make_float2(mean, rstd);
+    }
+    if (p.block) {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        if (!cols.ok(c)) continue;  // (what N_post's bias left there stays out of the row's sums)
+        if (GATE != GATE_NONE) {
+          float gv[V];
+          if (GATE == GATE_SHARED) {
+            kept.read(P::GATE_V, c, gv);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) gv[e] = 0.f;
+            if (live) in.read(p.in_gate, c, p.gate, w.at, cols, gv);
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) u[c][e] *= gv[e];
         }
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[c][e] += p.scale * u[c][e];
       }
     }
     if (p.sum && live) {
 #pragma unroll
       for (int c = 0; c < N; ++c)
-        if (cols.ok(c)) store_vec<T, V>(p.sum, at + cols.at(c), r[c]);
+        if (cols.ok(c)) store_vec<T, V>(p.sum, w.at + cols.at(c), r[c]);
     }
     if (p.pre) {
       float mean, rstd;
       row_stats<LAYER>(r, cols, p, sum, mean, rstd);
-      affine<LAYER>(r, cols, p.pre_w, p.pre_b, type16<T>(), p.w_type == 0, mean, rstd);
       if (live) {
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-          if (cols.ok(c)) store_vec<T, V>(p.y, at + cols.at(c), r[c]);
-        if (p.stats && t == 0 && rank == 0) *reinterpret_cast<float2*>(p.stats + row * 4 + 2) = make_float2(mean, rstd);
+        for (int c = 0; c < N; ++c) {
+          if (!cols.ok(c)) continue;
+          float wv[V], bv[V];
+          kept.read(P::PRE_W, c, wv);
+          if (LAYER) kept.read(P::PRE_B, c, bv);
+#pragma unroll
+          for (int e = 0; e < V; ++e) r[c][e] = LAYER ? (r[c][e] - mean) * rstd * wv[e] + bv[e] : r[c][e] * rstd * wv[e];
+          store_vec<T, V>(p.y, w.at + cols.at(c), r[c]);
+        }
+        if (p.stats && t == 0 && rank == 0) *reinterpret_cast<float2*>(p.stats + w.row * 4 + 2) = make_float2(mean, rstd);
       }
     }
+    new_gate = w.next(p);
   }
 }
 
 // Adds one array of column sums over the row groups of a block and writes the block's line of partial sums.
-template <int N, int V>
-__device__ __forceinline__ void flush_block(float (&acc)[N][V], const Cols<V>& cols, float* line, float* buf, int t, int group, int groups, int tpr) {
+template <int N, int V, bool FULL>
+__device__ __forceinline__ void flush_block(float (&acc)[N][V], const Cols<V, FULL>& cols, float* line, float* buf, int t, int group, int groups, int tpr) {
   if (groups == 1) {
 #pragma unroll
     for (int c = 0; c < N; ++c)
@@ -276,96 +386,118 @@ __device__ __forceinline__ void flush_block(float (&acc)[N][V], const Cols<V>& c
   }
 }
 
-template <typename T, int V, bool LAYER, bool POST, bool GATE, int E>
+template <typename T, int V, bool LAYER, bool POST, int GATE, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ NormParams p) {
-  constexpr int N = E / V;
-  __shared__ float red[64], peers[32], buf[128];
+  constexpr int N = bwd_elems<T, LAYER, POST, GATE>() / V;
+  using A = Ahead<T, V, N, FULL>;
+  using P = Places<LAYER, POST, GATE, true>;
+  __shared__ float red[GROUPS][64], peers[32], buf[SHARED_CTA];
   extern __shared__ __align__(16) uint8_t smem[];
   const int t = threadIdx.x & (p.tpr - 1), group = threadIdx.x >> p.tpr_log, groups = blockDim.x >> p.tpr_log;
   const int rank = blockIdx.x % p.cluster;
-  RowSum sum{red, peers, p.tpr, p.cluster, rank, 0};
-  const Cols<V> cols{(rank * N * p.tpr + t) * V, p.tpr * V, p.width};
+  RowSum sum{red[group & (GROUPS - 1)], peers, p.tpr, p.cluster, rank, group, 0};
+  const Cols<V, FULL> cols{(rank * N * p.tpr + t) * V, p.tpr * V, p.width};
   const long long team = blockIdx.x / p.cluster, worker = team * groups + group;
-  const long long first = min(worker * p.per_worker, p.rows), last = min(first + p.per_worker, p.rows);
+  Walk w(p, worker);
+  const long long first = w.row;
   float dw[N][V], db[N][V], dpw[N][V], dpb[N][V], dg[N][V];
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = dpw[c][e] = dpb[c][e] = dg[c][e] = 0.f;
-  Ahead<T, V, N> in(p, smem);
-  constexpr int STAGES = Ahead<T, V, N>::STAGES;
-  auto fetch = [&](int ahead, long long row) {
-    const bool live = row < last;
-    in.fetch(ahead, p.in_dy, p.dy, row * p.width, live, cols);
-    in.fetch(ahead, p.in_x, p.x, row * p.width, live, cols);
-    in.fetch(ahead, p.in_block, p.block, row * p.width, live, cols);
-    in.fetch(ahead, p.in_dsum, p.dsum, row * p.width, live, cols);
+  A in(p, smem);
+  const Kept<V, N, FULL> kept(smem + (V == 1 ? 0 : A::STAGES * p.n_in * N * 16 * (int)blockDim.x));
+  long long to_fetch = w.last - w.row, fetch_at = w.at + cols.first;
+  auto fetch = [&](int st) {
+    if (to_fetch > 0) {
+      in.fetch(st, p.in_dy, p.dy, fetch_at, cols);
+      in.fetch(st, p.in_x, p.x, fetch_at, cols);
+      in.fetch(st, p.in_block, p.block, fetch_at, cols);
+      in.fetch(st, p.in_dsum, p.dsum, fetch_at, cols);
+      if (GATE == GATE_ROWS) in.fetch(st, p.in_gate, p.gate, fetch_at, cols);
+      fetch_at += p.width;
+      --to_fetch;
+    }
     in.commit();
   };
-  for (int i = 0; i < STAGES - 1; ++i) fetch(i, first + i);
-
+  for (int i = 0; i < A::STAGES - 1; ++i) fetch(i);
+  const float4* stats_at = reinterpret_cast<const float4*>(p.stats) + w.row;
+  float4 st_next = w.live() ? __ldg(stats_at) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool w32 = p.w_type == 0, g32 = p.gate_type == 0;
+  if (p.dy) kept.keep(P::PRE_W, p.pre_w, 0, w32, type16<T>(), 1.f, cols);
+  if (POST) {
+    kept.keep(P::POST_W, p.post_w, 0, w32, type16<T>(), 1.f, cols);
+    if (LAYER) kept.keep(P::POST_B, p.post_b, 0, w32, type16<T>(), 0.f, cols);
+  }
+  auto read_gate = [&](int c, float (&gv)[V]) {
+    if (GATE == GATE_SHARED) kept.read(P::GATE_V, c, gv);
+    else in.read(p.in_gate, c, p.gate, w.at, cols, gv);
+  };
+  bool new_gate = true;
   for (long long i = 0; i < p.per_worker; ++i, in.next()) {  // (the same trips for all threads)
-    const long long row = first + i;
-    const bool live = row < last;
-    const long long at = row * p.width;
+    const bool live = w.live();
     float g[N][V], hat[N][V], u[N][V];
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) st = __ldg(reinterpret_cast<const float4*>(p.stats + row * 4));
-    fetch(STAGES - 1, row + STAGES - 1);
-    const long long gate_row = GATE && live ? row / p.per_gate : 0;
+    const float4 st = st_next;
+    if (w.row + 1 < w.last) st_next = __ldg(++stats_at);
+    fetch(in.free_stage());
+    if (GATE == GATE_SHARED && live && new_gate) kept.keep(P::GATE_V, p.gate, w.gate_row * p.width, g32, type16<T>(), 0.f, cols);
     in.ready();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
+      if (!live || !cols.ok(c)) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) g[c][e] = hat[c][e] = u[c][e] = 0.f;
-      if (!live || !cols.ok(c)) continue;
+        for (int e = 0; e < V; ++e) g[c][e] = hat[c][e] = u[c][e] = 0.f;
+        continue;
+      }
       // the sum again, as the forward pass had it before rounding
       if (p.block) {
-        in.read(p.in_block, c, p.block, at, cols, u[c]);
+        in.read(p.in_block, c, p.block, w.at, cols, u[c]);
+        if (POST) {
+          float wv[V], bv[V];
+          kept.read(P::POST_W, c, wv);
+          if (LAYER) kept.read(P::POST_B, c, bv);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          if (POST) u[c][e] = LAYER ? (u[c][e] - st.x) * st.y : u[c][e] * st.y;
-          hat[c][e] = u[c][e];
-        }
-        if (POST && p.post_w) {
-          float wv[V];
-          load_param<V>(p.post_w, cols.at(c), p.w_type == 0, type16<T>(), wv);
+          for (int e = 0; e < V; ++e) {
+            u[c][e] = LAYER ? (u[c][e] - st.x) * st.y : u[c][e] * st.y;
+            hat[c][e] = LAYER ? u[c][e] * wv[e] + bv[e] : u[c][e] * wv[e];
+          }
+        } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) hat[c][e] *= wv[e];
+          for (int e = 0; e < V; ++e) hat[c][e] = u[c][e];
         }
-        if (POST && LAYER && p.post_b) {
-          float bv[V];
-          load_param<V>(p.post_b, cols.at(c), p.w_type == 0, type16<T>(), bv);
-#pragma unroll
-          for (int e = 0; e < V; ++e) hat[c][e] += bv[e];
-        }
-        if (GATE) {
+        if (GATE != GATE_NONE) {
           float gv[V];
-          load_param<V>(p.gate, gate_row * p.width + cols.at(c), p.gate_type == 0, type16<T>(), gv);
+          read_gate(c, gv);
 #pragma unroll
           for (int e = 0; e < V; ++e) hat[c][e] *= gv[e];
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) hat[c][e] = u[c][e] = 0.f;
       }
       if (p.dy) {
         float xv[V], wv[V];
-        in.read(p.in_x, c, p.x, at, cols, xv);
-        in.read(p.in_dy, c, p.dy, at, cols, g[c]);
-        if (p.pre_w) load_param<V>(p.pre_w, cols.at(c), p.w_type == 0, type16<T>(), wv);
+        in.read(p.in_x, c, p.x, w.at, cols, xv);
+        in.read(p.in_dy, c, p.dy, w.at, cols, g[c]);
+        kept.read(P::PRE_W, c, wv);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float r = xv[e] + p.scale * hat[c][e];
           hat[c][e] = LAYER ? (r - st.z) * st.w : r * st.w;
           dw[c][e] += g[c][e] * hat[c][e];
           if (LAYER) db[c][e] += g[c][e];
-          if (p.pre_w) g[c][e] *= wv[e];
+          g[c][e] *= wv[e];
           if (LAYER) s1 += g[c][e];
           s2 += g[c][e] * hat[c][e];
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[c][e] = 0.f;
       }
     }
     if (p.dy) {
-      sum(s1, s2, true);
+      sum(LAYER ? s1 : s2, LAYER ? s2 : s1, LAYER);
       s1 *= p.inv_width;
       s2 *= p.inv_width;
 #pragma unroll
@@ -379,14 +511,14 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
         if (!cols.ok(c)) continue;
         if (p.dsum) {
           float dr[V];
-          in.read(p.in_dsum, c, p.dsum, at, cols, dr);
+          in.read(p.in_dsum, c, p.dsum, w.at, cols, dr);
 #pragma unroll
           for (int e = 0; e < V; ++e) g[c][e] += dr[e];
         }
-        store_vec<T, V>(p.dx, at + cols.at(c), g[c]);
+        store_vec<T, V>(p.dx, w.at + cols.at(c), g[c]);
       }
     }
-    if (!POST && !GATE) {
+    if (!POST && GATE == GATE_NONE) {
       if (p.dblock && live) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
@@ -394,9 +526,10 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
             float d[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) d[e] = p.scale * g[c][e];
-            store_vec<T, V>(p.dblock, at + cols.at(c), d);
+            store_vec<T, V>(p.dblock, w.at + cols.at(c), d);
           }
       }
+      w.next(p);
       continue;
     }
     s1 = s2 = 0.f;
@@ -404,23 +537,18 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
     for (int c = 0; c < N; ++c) {
       if (!live || !cols.ok(c)) continue;
       float wv[V], bv[V], gv[V];
-      if (POST && p.post_w) load_param<V>(p.post_w, cols.at(c), p.w_type == 0, type16<T>(), wv);
-      if (POST && GATE && LAYER && p.post_b) load_param<V>(p.post_b, cols.at(c), p.w_type == 0, type16<T>(), bv);
-      if (GATE) load_param<V>(p.gate, gate_row * p.width + cols.at(c), p.gate_type == 0, type16<T>(), gv);
+      if (POST) kept.read(P::POST_W, c, wv);
+      if (POST && GATE != GATE_NONE && LAYER) kept.read(P::POST_B, c, bv);
+      if (GATE != GATE_NONE) read_gate(c, gv);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float h = u[c][e], d = p.scale * g[c][e];
-        if (GATE) {
-          float v = h;
-          if (POST && p.post_w) v *= wv[e];
-          if (POST && LAYER && p.post_b) v += bv[e];
-          dg[c][e] += v * d;
-        }
-        float du = GATE ? d * gv[e] : d;
+        if (GATE != GATE_NONE) dg[c][e] += (!POST ? h : LAYER ? h * wv[e] + bv[e] : h * wv[e]) * d;
+        float du = GATE != GATE_NONE ? d * gv[e] : d;
         if (POST) {
           dpw[c][e] += du * h;
           if (LAYER) dpb[c][e] += du;
-          if (p.post_w) du *= wv[e];
+          du *= wv[e];
           if (LAYER) s1 += du;
           s2 += du * h;
         }
@@ -428,7 +556,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
       }
     }
     if (POST) {
-      sum(s1, s2, true);
+      sum(LAYER ? s1 : s2, LAYER ? s2 : s1, LAYER);
       s1 *= p.inv_width;
       s2 *= p.inv_width;
 #pragma unroll
@@ -439,17 +567,17 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
     if (p.dblock && live) {
 #pragma unroll
       for (int c = 0; c < N; ++c)
-        if (cols.ok(c)) store_vec<T, V>(p.dblock, at + cols.at(c), g[c]);
+        if (cols.ok(c)) store_vec<T, V>(p.dblock, w.at + cols.at(c), g[c]);
     }
-    if (GATE && live && p.dgate && (row + 1 == last || (row + 1) / p.per_gate != gate_row)) {
-      const long long begin = gate_row * p.per_gate;
-      const bool whole = begin >= first && begin + p.per_gate <= last;
+    if (GATE != GATE_NONE && live && p.dgate && (w.row + 1 == w.last || w.gate_left == 1)) {
+      const long long begin = w.gate_row * p.per_gate;
+      const bool whole = begin >= first && begin + p.per_gate <= w.last;
       float* slot = p.gate_part + (worker * 2 + (begin < first ? 0 : 1)) * p.width;
 #pragma unroll
       for (int c = 0; c < N; ++c) {
         if (!cols.ok(c)) continue;
         if (whole) {
-          store_param<V>(p.dgate, gate_row * p.width + cols.at(c), p.gate_type == 0, type16<T>(), dg[c]);
+          store_param<V>(p.dgate, w.gate_row * p.width + cols.at(c), g32, type16<T>(), dg[c]);
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) slot[cols.at(c) + e] = dg[c][e];
@@ -458,6 +586,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
         for (int e = 0; e < V; ++e) dg[c][e] = 0.f;
       }
     }
+    new_gate = w.next(p);
   }
   float* line = p.part + team * 4 * p.width;
   if (p.dpre_w) flush_block(dw, cols, line, buf, t, group, groups, p.tpr);
@@ -466,11 +595,13 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
   if (POST && LAYER && p.dpost_b) flush_block(dpb, cols, line + 3 * p.width, buf, t, group, groups, p.tpr);
 }
 
-// blockIdx.y < 4: sums a weight's or bias's lines over the teams; then one block for each worker that takes over a group of the
-// gate from the worker before it, where that group began: sums the group's slots.  32 columns x 32 consecutive shares.
+// blockIdx.y < 4: sums a weight's or bias's lines over the teams.  Then the rows of the gate that several workers share, each the sum of
+// its slots: one block for each row of the gate, or, where there are more of those than workers, for each worker that takes
+// over a row from the one before it, where that row began.  32 columns x 16 consecutive shares.
+constexpr int SHARES = 16;
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_reduce(const __grid_constant__ NormParams p, int teams) {
-  __shared__ float part[32][33];
+__global__ void __launch_bounds__(32 * SHARES) norm_reduce(const __grid_constant__ NormParams p, int teams, int by_worker) {
+  __shared__ float part[SHARES][33];
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
   const bool ok = col < p.width;
   float s = 0.f;
@@ -480,21 +611,24 @@ __global__ void __launch_bounds__(1024) norm_reduce(const __grid_constant__ Norm
   if (blockIdx.y < 4) {
     out = blockIdx.y == 0 ? p.dpre_w : blockIdx.y == 1 ? p.dpre_b : blockIdx.y == 2 ? p.dpost_w : p.dpost_b;
     if (!out) return;
-    const int per = (teams + 31) / 32, end = min(teams, (share + 1) * per);
+    const int per = (teams + SHARES - 1) / SHARES, end = min(teams, (share + 1) * per);
     const float* at = p.part + (long long)blockIdx.y * p.width + col;
 #pragma unroll 8
     for (int i = share * per; i < end; ++i) s += ok ? __ldcg(at + (long long)i * 4 * p.width) : 0.f;
   } else {
-    const long long w = (long long)blockIdx.y - 4 + 1;
-    if (w >= p.workers) return;
-    const long long row = w * p.per_worker;
-    if (row >= p.rows || row % p.per_gate == 0) return;
-    const long long g = row / p.per_gate, begin = g * p.per_gate;
-    if (begin / p.per_worker != w - 1) return;
-    const long long w1 = (begin + p.per_gate - 1) / p.per_worker, n = w1 - w + 2;  // slots: the second of w - 1, the first of w .. w1
-    const long long per = (n + 31) / 32, end = min(n, (share + 1) * per);
+    const long long item = (long long)blockIdx.y - 4;
+    long long g = item;
+    if (by_worker) {
+      const long long row = (item + 1) * p.per_worker;
+      if (row >= p.rows || row % p.per_gate == 0) return;
+      g = row / p.per_gate;
+      if (g * p.per_gate / p.per_worker != item) return;
+    }
+    const long long begin = g * p.per_gate, w0 = begin / p.per_worker, w1 = (begin + p.per_gate - 1) / p.per_worker, n = w1 - w0 + 1;
+    if (n == 1) return;
+    const long long per = (n + SHARES - 1) / SHARES, end = min(n, (share + 1) * per);  // slots: the second of w0, the first of the others
 #pragma unroll 4
-    for (long long i = share * per; i < end; ++i) s += ok ? __ldcg(p.gate_part + ((w - 1 + i) * 2 + (i == 0 ? 1 : 0)) * p.width + col) : 0.f;
+    for (long long i = share * per; i < end; ++i) s += ok ? __ldcg(p.gate_part + ((w0 + i) * 2 + (i == 0 ? 1 : 0)) * p.width + col) : 0.f;
     out = p.dgate;
     out_at = g * p.width + col;
     f32 = p.gate_type == 0;
@@ -503,7 +637,7 @@ __global__ void __launch_bounds__(1024) norm_reduce(const __grid_constant__ Norm
   __syncthreads();
   if (share == 0 && ok) {
     float v[1] = {0.f};
-    for (int i = 0; i < 32; ++i) v[0] += part[i][threadIdx.x & 31];
+    for (int i = 0; i < SHARES; ++i) v[0] += part[i][threadIdx.x & 31];
     store_param<1>(out, out_at, f32, type16<T>(), v);
   }
 }
@@ -522,7 +656,7 @@ struct Shape {
   int e, tpr, tpr_log, cluster, threads;
 };
 
-// Threads per row: enough for E elements each, at least 4; rows of up to 32 threads share CTAs of 128.
+// Threads per row: enough for E elements each, at least 4; rows of up to 128 threads share CTAs of 256.
 static bool shape_of(int width, int e, Shape* s) {
   s->e = e;
   s->cluster = 1;
@@ -531,16 +665,9 @@ static bool shape_of(int width, int e, Shape* s) {
   s->tpr = 4;
   s->tpr_log = 2;
   while ((long long)s->tpr * e * s->cluster < width) s->tpr *= 2, ++s->tpr_log;
-  s->threads = s->tpr > 128 ? s->tpr : 128;
-  if (s->tpr > 32) s->threads = s->tpr;
+  s->threads = s->tpr > SHARED_CTA ? s->tpr : SHARED_CTA;
   return true;
 }
-
-// Elements per thread.  Backward passes through N_post or a gate keep five arrays of column sums: 8 elements fit 128 registers;
-// four FP32 tensors of 16 elements for 512 threads, two stages, do not fit shared memory.
-template <typename T>
-constexpr int bwd_elems(bool post, bool gate) { return post || gate || sizeof(T) == 4 ? 8 : 16; }
-constexpr int FWD_ELEMS = 16;
 
 struct Plan {
   Shape s;
@@ -549,12 +676,12 @@ struct Plan {
   size_t part_bytes, gate_bytes;
 };
 
-static bool bwd_plan(long long rows, int width, bool post, bool gate, int dtype, int device, Plan* pl) {
-  if (!shape_of(width, dtype == 0 ? bwd_elems<float>(post, gate) : bwd_elems<__half>(post, gate), &pl->s)) return false;
+// Consecutive rows for each worker: as many CTAs as stay resident (`resident` threads a multiprocessor), at least `least` rows a worker.
+static bool make_plan(long long rows, int width, int elems, int resident, int least, bool gate, int device, Plan* pl) {
+  if (!shape_of(width, elems, &pl->s)) return false;
   pl->groups = pl->s.threads / pl->s.tpr;
-  // as many CTAs as stay resident (128 registers a thread), and at least four rows for a worker: each leaves a line of sums
-  long long teams = (long long)host_sm_count(device) * (512 / pl->s.threads) / pl->s.cluster;
-  const long long most = (rows + 4LL * pl->groups - 1) / (4LL * pl->groups);
+  long long teams = (long long)host_sm_count(device) * (resident / pl->s.threads) / pl->s.cluster;
+  const long long most = (rows + (long long)least * pl->groups - 1) / ((long long)least * pl->groups);
   if (teams > most) teams = most;
   if (teams < 1) teams = 1;
   pl->per_worker = (rows + teams * pl->groups - 1) / (teams * pl->groups);
@@ -566,6 +693,10 @@ static bool bwd_plan(long long rows, int width, bool post, bool gate, int dtype,
   pl->gate_bytes = gate ? (size_t)pl->workers * 2 * width * sizeof(float) : 0;
   return true;
 }
+// (backward: each worker leaves a line of column sums, so at least four rows)
+static bool bwd_plan(long long rows, int width, bool post, bool gate, int dtype, int device, Plan* pl) {
+  return make_plan(rows, width, post || gate || dtype == 0 ? 8 : 16, 512, 4, gate, device, pl);
+}
 
 static bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -574,48 +705,70 @@ static bool vector_ok(const NormParams& p, int v) {
          aligned(p.pre_b) && aligned(p.sum) && aligned(p.y) && aligned(p.dsum) && aligned(p.dy) && aligned(p.dx) && aligned(p.dblock) && aligned(p.dgate);
 }
 
-// The bytes of a CTA's fetched-ahead rows: `elems` elements a thread of each tensor.
-template <typename T, int V>
-static int ahead_bytes(const NormParams& p, int elems, int threads) {
-  return V == 1 ? 0 : Ahead<T, V, 1>::STAGES * p.n_in * elems * (int)sizeof(T) * threads;
-}
-
 template <typename K>
-static cudaError_t launch(K kernel, unsigned grid, int threads, int cluster, int smem, cudaStream_t st, const NormParams& p) {
-  if (smem > 40 * 1024) {  // (48 KB with the static arrays; per device and kernel; a call that raises it again costs under a microsecond)
+static cudaError_t launch(K kernel, const Plan& pl, int smem, cudaStream_t st, const NormParams& p) {
+  if (smem > 40 * 1024) {  // (48 KB with the static arrays)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
+  cfg.gridDim = dim3((unsigned)(pl.teams * pl.s.cluster));
+  cfg.blockDim = dim3(pl.s.threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = cluster;
+  at.val.clusterDim.x = pl.s.cluster;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.numAttrs = pl.s.cluster > 1 ? 1 : 0;
   host_count_launch();
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <typename T, int V>
-static cudaError_t fwd_launch(const NormParams& p, bool layer, unsigned grid, const Shape& s, cudaStream_t st) {
-  const int smem = ahead_bytes<T, V>(p, FWD_ELEMS, s.threads);
-  return layer ? launch(norm_fwd<T, V, true, FWD_ELEMS>, grid, s.threads, s.cluster, smem, st, p)
-               : launch(norm_fwd<T, V, false, FWD_ELEMS>, grid, s.threads, s.cluster, smem, st, p);
+// Shared memory of a CTA: the rows on their way and the kept arrays.
+template <typename T, int V, int KEPT>
+static int smem_bytes(const NormParams& p, int elems, int threads) {
+  return (V == 1 ? 0 : (sizeof(T) == 4 ? 2 : 3) * p.n_in * elems * (int)sizeof(T) * threads) + KEPT * elems * 4 * threads;
+}
+
+template <typename T, int V, bool LAYER, bool POST, int GATE>
+static cudaError_t launch_t(NormParams& p, bool backward, int device, cudaStream_t st, const Plan* bwd) {
+  if (backward) {
+    constexpr int E = bwd_elems<T, LAYER, POST, GATE>();
+    const int smem = smem_bytes<T, V, Places<LAYER, POST, GATE, true>::COUNT>(p, E, bwd->s.threads);
+    if (V > 1 && p.width == bwd->s.tpr * E * bwd->s.cluster) return launch(norm_bwd<T, V, LAYER, POST, GATE, (V > 1)>, *bwd, smem, st, p);
+    return launch(norm_bwd<T, V, LAYER, POST, GATE, false>, *bwd, smem, st, p);
+  }
+  constexpr int E = fwd_elems<T, LAYER, POST, GATE>();
+  Plan pl;
+  if (!make_plan(p.rows, p.width, E, 512, 1, false, device, &pl)) return cudaErrorInvalidValue;
+  p.tpr = pl.s.tpr; p.tpr_log = pl.s.tpr_log; p.cluster = pl.s.cluster; p.per_worker = pl.per_worker; p.workers = pl.workers;
+  const int smem = smem_bytes<T, V, Places<LAYER, POST, GATE, false>::COUNT>(p, E, pl.s.threads);
+  if (V > 1 && p.width == pl.s.tpr * E * pl.s.cluster) return launch(norm_fwd<T, V, LAYER, POST, GATE, (V > 1)>, pl, smem, st, p);
+  return launch(norm_fwd<T, V, LAYER, POST, GATE, false>, pl, smem, st, p);
 }
 
 template <typename T, int V, bool LAYER>
-static cudaError_t bwd_launch(const NormParams& p, bool post, bool gate, const Plan& pl, cudaStream_t st) {
-  const unsigned grid = (unsigned)(pl.teams * pl.s.cluster);
-  const int smem = ahead_bytes<T, V>(p, pl.s.e, pl.s.threads);
-  if (post && gate) return launch(norm_bwd<T, V, LAYER, true, true, 8>, grid, pl.s.threads, pl.s.cluster, smem, st, p);
-  if (post) return launch(norm_bwd<T, V, LAYER, true, false, 8>, grid, pl.s.threads, pl.s.cluster, smem, st, p);
-  if (gate) return launch(norm_bwd<T, V, LAYER, false, true, 8>, grid, pl.s.threads, pl.s.cluster, smem, st, p);
-  return launch(norm_bwd<T, V, LAYER, false, false, bwd_elems<T>(false, false)>, grid, pl.s.threads, pl.s.cluster, smem, st, p);
+static cudaError_t launch_l(NormParams& p, bool backward, bool post, int gate, int device, cudaStream_t st, const Plan* bwd) {
+  if (gate == GATE_ROWS) return post ? launch_t<T, V, LAYER, true, GATE_ROWS>(p, backward, device, st, bwd) : launch_t<T, V, LAYER, false, GATE_ROWS>(p, backward, device, st, bwd);
+  if (gate == GATE_SHARED) return post ? launch_t<T, V, LAYER, true, GATE_SHARED>(p, backward, device, st, bwd) : launch_t<T, V, LAYER, false, GATE_SHARED>(p, backward, device, st, bwd);
+  return post ? launch_t<T, V, LAYER, true, GATE_NONE>(p, backward, device, st, bwd) : launch_t<T, V, LAYER, false, GATE_NONE>(p, backward, device, st, bwd);
+}
+
+template <typename T, int V>
+static cudaError_t launch_v(NormParams& p, bool backward, bool layer, bool post, int gate, int device, cudaStream_t st, const Plan* bwd) {
+  return layer ? launch_l<T, V, true>(p, backward, post, gate, device, st, bwd) : launch_l<T, V, false>(p, backward, post, gate, device, st, bwd);
+}
+
+static cudaError_t dispatch(NormParams& p, bool backward, bool layer, bool post, int dtype, int device, cudaStream_t st, const Plan* bwd) {
+  // a gate of one row per row, of the activations' type, is fetched ahead like them
+  const int gate = !p.gate ? GATE_NONE : p.per_gate == 1 && p.gate_type == dtype ? GATE_ROWS : GATE_SHARED;
+  if (gate == GATE_ROWS) p.in_gate = p.n_in++;
+  const bool vec = vector_ok(p, dtype == 0 ? 4 : 8);
+  if (dtype == 0) return vec ? launch_v<float, 4>(p, backward, layer, post, gate, device, st, bwd) : launch_v<float, 1>(p, backward, layer, post, gate, device, st, bwd);
+  if (dtype == 1) return vec ? launch_v<__nv_bfloat16, 8>(p, backward, layer, post, gate, device, st, bwd) : launch_v<__nv_bfloat16, 1>(p, backward, layer, post, gate, device, st, bwd);
+  return vec ? launch_v<__half, 8>(p, backward, layer, post, gate, device, st, bwd) : launch_v<__half, 1>(p, backward, layer, post, gate, device, st, bwd);
 }
 
 template <typename T>
@@ -623,10 +776,11 @@ static cudaError_t reduce_launch(const NormParams& p, const Plan& pl, cudaStream
   const bool weights = p.dpre_w || p.dpre_b || p.dpost_w || p.dpost_b;
   const bool gates = p.dgate != nullptr && pl.workers > 1;
   if (!weights && !gates) return cudaSuccess;
-  const long long items = gates ? pl.workers - 1 : 0;
-  const dim3 grid((p.width + 31) / 32, (unsigned)(4 + items));  // (items: at most 4 x 32 workers a multiprocessor: 18944 of 65531)
+  const long long gate_rows = p.rows / p.per_gate;
+  const int by_worker = gate_rows > pl.workers - 1;
+  const long long items = !gates ? 0 : by_worker ? pl.workers - 1 : gate_rows;  // (at most 2 x 64 workers a multiprocessor: 18944 of 65531)
   host_count_launch();
-  norm_reduce<T><<<grid, 1024, 0, st>>>(p, (int)pl.teams);
+  norm_reduce<T><<<dim3((p.width + 31) / 32, (unsigned)(4 + items)), 32 * SHARES, 0, st>>>(p, (int)pl.teams, by_worker);
   return cudaGetLastError();
 }
 
@@ -668,24 +822,10 @@ int amsim_residual_norm(void* stream, const void* x, const void* block, const vo
   p.sum = sum; p.y = y; p.stats = stats;
   p.rows = rows; p.per_gate = gate ? rows / gate_rows : 1; p.width = width;
   p.w_type = w_dtype; p.gate_type = gate_dtype; p.scale = scale; p.eps = eps; p.inv_width = 1.f / (float)width;
-  p.post = post; p.pre = pre;
+  p.pre = pre;
   p.in_x = p.n_in++;
   if (block) p.in_block = p.n_in++;
-  Shape s;
-  if (!shape_of(width, FWD_ELEMS, &s)) return host_fail(AMSIM_ERR_UNSUPPORTED, "residual norm: width");
-  p.tpr = s.tpr; p.tpr_log = s.tpr_log; p.cluster = s.cluster;
-  const int groups = s.threads / s.tpr;
-  long long teams = (rows + groups - 1) / groups;
-  const long long most = (long long)host_sm_count(host_device()) * 32 / s.cluster;  // (more CTAs than stay resident: they balance the last rows)
-  if (teams > most) teams = most;
-  const unsigned grid = (unsigned)(teams * s.cluster);
-  cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = vector_ok(p, dtype == 0 ? 4 : 8);
-  cudaError_t e;
-  if (dtype == 0) e = vec ? fwd_launch<float, 4>(p, layer, grid, s, st) : fwd_launch<float, 1>(p, layer, grid, s, st);
-  else if (dtype == 1) e = vec ? fwd_launch<__nv_bfloat16, 8>(p, layer, grid, s, st) : fwd_launch<__nv_bfloat16, 1>(p, layer, grid, s, st);
-  else e = vec ? fwd_launch<__half, 8>(p, layer, grid, s, st) : fwd_launch<__half, 1>(p, layer, grid, s, st);
-  AMSIM_HOST_TRY(e);
+  AMSIM_HOST_TRY(dispatch(p, false, layer, post, dtype, host_device(), (cudaStream_t)stream, nullptr));
   return AMSIM_OK;
 }
 
@@ -715,7 +855,7 @@ int amsim_residual_norm_grad(void* stream, const void* dsum, const void* dy, con
   p.dx = dx; p.dblock = dblock; p.dgate = dgate; p.dpost_w = dpost_w; p.dpost_b = dpost_b; p.dpre_w = dpre_w; p.dpre_b = dpre_b;
   p.rows = rows; p.per_gate = gate ? rows / gate_rows : 1; p.width = width;
   p.w_type = w_dtype; p.gate_type = gate_dtype; p.scale = scale; p.inv_width = 1.f / (float)width;
-  p.post = post; p.pre = pre;
+  p.pre = pre;
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) {
     const dim3 grid((width + 255) / 256, 4);
@@ -745,16 +885,8 @@ int amsim_residual_norm_grad(void* stream, const void* dsum, const void* dy, con
   if (!dy && !post && !gate) p.block = nullptr;
   if (p.block) p.in_block = p.n_in++;
   if (dsum) p.in_dsum = p.n_in++;
-  const bool vec = vector_ok(p, dtype == 0 ? 4 : 8);
-  cudaError_t e;
-#define AMSIM_BWD(T, V) (layer ? bwd_launch<T, V, true>(p, post, gate != nullptr, pl, st) : bwd_launch<T, V, false>(p, post, gate != nullptr, pl, st))
-  if (dtype == 0) e = vec ? AMSIM_BWD(float, 4) : AMSIM_BWD(float, 1);
-  else if (dtype == 1) e = vec ? AMSIM_BWD(__nv_bfloat16, 8) : AMSIM_BWD(__nv_bfloat16, 1);
-  else e = vec ? AMSIM_BWD(__half, 8) : AMSIM_BWD(__half, 1);
-#undef AMSIM_BWD
-  AMSIM_HOST_TRY(e);
-  e = dtype == 0 ? reduce_launch<float>(p, pl, st) : dtype == 1 ? reduce_launch<__nv_bfloat16>(p, pl, st) : reduce_launch<__half>(p, pl, st);
-  AMSIM_HOST_TRY(e);
+  AMSIM_HOST_TRY(dispatch(p, true, layer, post, dtype, host_device(), st, &pl));
+  AMSIM_HOST_TRY(dtype == 0 ? reduce_launch<float>(p, pl, st) : dtype == 1 ? reduce_launch<__nv_bfloat16>(p, pl, st) : reduce_launch<__half>(p, pl, st));
   return AMSIM_OK;
 }
 
