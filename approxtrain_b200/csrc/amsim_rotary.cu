@@ -6,7 +6,8 @@
 // Bound by memory: one read and one write of each element.  Far positions need the angle to more than FP32 holds (at 10^6 an
 // FP32 angle is off by 0.06): p f_i / 2 pi is taken in 64 bits, its whole turns dropped, and the rest of a turn goes through
 // sincospif, whose argument is then exact to 2^-25 turns.  A CTA does that once per token and pair, for all heads of both
-// tensors, into shared memory; its first elements are already on their way meanwhile.
+// tensors, into shared memory.  A thread keeps its place within the head (a 16-byte chunk, or two that turn together)
+// and walks over the heads of the CTA's tokens, so nothing is divided on the way and neighbours touch neighbouring chunks.
 #include "amsim_elem.cuh"
 #include "amsim_host.h"
 
@@ -14,18 +15,8 @@ namespace amsim {
 namespace rotary {
 
 constexpr int THREADS = 256;
-constexpr int UNROLL = 4;             // units of a thread in flight
 constexpr int MAX_PAIRS = 4096;       // angles of a CTA: 32 KB
-
-struct Div {  // n / d for n < 2^31 by a multiplication
-  uint32_t mul, shift, d;
-};
-static Div make_div(uint32_t d) {
-  uint32_t s = 0;
-  while ((1u << s) < d) ++s;
-  return {(uint32_t)((((1ull << 32) * ((1ull << s) - d)) / d) + 1), s, d};
-}
-__device__ __forceinline__ uint32_t quot(uint32_t n, const Div& v) { return (__umulhi(n, v.mul) + n) >> v.shift; }
+constexpr int MAX_TOKENS = 64;        // tokens of a CTA
 
 struct Side {           // one tensor: its heads at x + b xb + s xs + h xh (elements), the last axis dense
   const void* x;
@@ -37,119 +28,131 @@ struct Params {
   Side side[2];
   const void* positions;
   const double* freqs;
-  long long pos_b, pos_s, tokens;
-  Div seq, units, heads;               // units of a head; heads of both tensors
-  int heads0, half, rot, n_rot;        // n_rot: units that are rotated, the rest are copied
-  int tokens_per_cta, pos32, interleaved;
+  long long pos_b, pos_s, tokens, seq;
+  int heads, heads0;                   // of both tensors, of the first
+  int half, rot, n_rot, units;         // chunks of a head that turn, and all of them
+  int tokens_per_cta, pos32;
   float scale, sign;
 };
 
+// A chunk as it is loaded: 16 bytes, or one element.
 template <typename T, int V>
-struct Unit {
-  float a[V], b[V];
+struct Chunk {
+  using type = uint4;
+  __device__ static __forceinline__ void unpack(const uint4& c, float (&o)[V]) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    unpack16<T, V>(w, o);
+  }
+};
+template <typename T>
+struct Chunk<T, 1> {
+  using type = T;
+  __device__ static __forceinline__ void unpack(const T& c, float (&o)[1]) { o[0] = elem_to_float(c); }
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) rotate(const __grid_constant__ Params p) {
-  __shared__ float2 turn[MAX_PAIRS];
+// V elements a chunk.  HALF: a chunk of the first half turns with the one half behind it; else a chunk holds V / 2 pairs (V = 1: two
+// adjacent elements).
+template <typename T, int V, bool HALF>
+__global__ void __launch_bounds__(THREADS, 3) rotate(const __grid_constant__ Params p) {
+  constexpr bool TWO = HALF || V == 1;           // a turning chunk is two loads
+  constexpr int PAIRS = TWO ? V : V / 2;         // pairs of a turning chunk
+  constexpr int UNROLL = TWO ? 4 : 8;            // heads of a thread in flight
+  using Raw = typename Chunk<T, V>::type;
+  __shared__ __align__(16) float2 turn[MAX_PAIRS];
+  __shared__ long long in_at[2][MAX_TOKENS], out_at[2][MAX_TOKENS];
+  __shared__ double pos[MAX_TOKENS];
   const long long token0 = (long long)blockIdx.x * p.tokens_per_cta;
   const int tokens = (int)min((long long)p.tokens_per_cta, p.tokens - token0);
-  const uint32_t all = (uint32_t)tokens * p.heads.d * p.units.d;
+  for (int i = threadIdx.x; i < tokens; i += THREADS) {
+    const long long t = token0 + i, b = t / p.seq, s = t - b * p.seq, where = b * p.pos_b + s * p.pos_s;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      in_at[k][i] = b * p.side[k].xb + s * p.side[k].xs;
+      out_at[k][i] = b * p.side[k].ob + s * p.side[k].os;
+    }
+    pos[i] = p.pos32 ? (double)static_cast<const int*>(p.positions)[where] : (double)static_cast<const long long*>(p.positions)[where];
+  }
+  __syncthreads();
 
-  struct Place {
-    const T* x;
-    T* out;
-    int tok, unit;
+  const int wide = min(p.units, THREADS), lanes = THREADS / wide, lane = threadIdx.x / wide, rows = lane < lanes ? tokens * p.heads : 0;
+  int unit = threadIdx.x - lane * wide, row = lane, tok = lane / p.heads, head = lane - tok * p.heads;
+  bool turns = false;
+  int first = 0, second = 0;
+  auto begin_unit = [&]() {
+    turns = unit < p.n_rot;
+    first = !turns ? p.rot + V * (unit - p.n_rot) : HALF ? V * unit : 2 * PAIRS * unit;
+    second = first + (HALF ? p.half : V);
   };
-  // unit number i of the CTA: its head's first element in both tensors
-  auto place = [&](uint32_t i) {
-    const uint32_t head_all = quot(i, p.units), unit = i - head_all * p.units.d;
-    const uint32_t tok = quot(head_all, p.heads);
-    uint32_t head = head_all - tok * p.heads.d;
-    const long long t = token0 + tok;
-    const long long b = p.tokens < (1ll << 31) ? quot((uint32_t)t, p.seq) : t / p.seq.d;
-    const long long s = t - b * p.seq.d;
-    const int which = head >= (uint32_t)p.heads0;
-    if (which) head -= p.heads0;
-    const Side& d = p.side[which];
-    return Place{static_cast<const T*>(d.x) + (b * d.xb + s * d.xs + head * d.xh), static_cast<T*>(d.out) + (b * d.ob + s * d.os + head * d.oh), (int)tok, (int)unit};
-  };
-  auto load = [&](const Place& at, Unit<T, V>& u) {
-    if (at.unit < p.n_rot) {
-      const int first = p.interleaved ? 2 * V * at.unit : V * at.unit;
-      load_vec<T, V>(at.x, first, u.a);
-      load_vec<T, V>(at.x, first + (p.interleaved ? V : p.half), u.b);
-    } else {
-      load_vec<T, V>(at.x, p.rot + V * (at.unit - p.n_rot), u.a);
+  begin_unit();
+  Raw a[UNROLL], b[TWO ? UNROLL : 1];
+  T* out[UNROLL];
+  int of[UNROLL];
+  auto load = [&]() {  // the next heads of this thread, as many as there are
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      if (row + k * lanes >= rows) break;
+      const int which = head >= p.heads0, h = which ? head - p.heads0 : head;
+      const Side& d = p.side[which];
+      const T* const x = static_cast<const T*>(d.x) + (in_at[which][tok] + h * d.xh);
+      out[k] = static_cast<T*>(d.out) + (out_at[which][tok] + h * d.oh);
+      of[k] = tok;
+      a[k] = *reinterpret_cast<const Raw*>(x + first);
+      if (TWO && turns) b[TWO ? k : 0] = *reinterpret_cast<const Raw*>(x + second);
+      for (head += lanes; head >= p.heads; head -= p.heads) ++tok;
     }
   };
-  auto finish = [&](const Place& at, Unit<T, V>& u) {
-    if (at.unit >= p.n_rot) {
-      store_vec<T, V>(at.out, p.rot + V * (at.unit - p.n_rot), u.a);
-      return;
-    }
-    const float2* cs = turn + at.tok * p.half + V * at.unit;
-    if (p.interleaved) {  // a, b: 2 V adjacent elements, V pairs
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float& x = 2 * e < V ? u.a[(2 * e) % V] : u.b[(2 * e) % V];
-        float& y = 2 * e + 1 < V ? u.a[(2 * e + 1) % V] : u.b[(2 * e + 1) % V];
-        const float2 c = cs[e];
-        const float r = x * c.x - y * c.y;
-        y = y * c.x + x * c.y;
-        x = r;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 c = cs[e];
-        const float r = u.a[e] * c.x - u.b[e] * c.y;
-        u.b[e] = u.b[e] * c.x + u.a[e] * c.y;
-        u.a[e] = r;
-      }
-    }
-    const int first = p.interleaved ? 2 * V * at.unit : V * at.unit;
-    store_vec<T, V>(at.out, first, u.a);
-    store_vec<T, V>(at.out, first + (p.interleaved ? V : p.half), u.b);
-  };
-
-  Place at[UNROLL];
-  Unit<T, V> u[UNROLL];
-  uint32_t i0 = threadIdx.x;
-  auto load_all = [&]() {
-#pragma unroll
-    for (int k = 0; k < UNROLL; ++k)
-      if (i0 + k * THREADS < all) {
-        at[k] = place(i0 + k * THREADS);
-        load(at[k], u[k]);
-      }
-  };
-  load_all();
+  load();  // (on their way while the angles are made)
   for (int i = threadIdx.x; i < tokens * p.half; i += THREADS) {
-    const int tok = i / p.half, pair = i - tok * p.half;
-    const long long t = token0 + tok, b = t / p.seq.d, s = t - b * p.seq.d, where = b * p.pos_b + s * p.pos_s;
-    const double pos = p.pos32 ? (double)static_cast<const int*>(p.positions)[where] : (double)static_cast<const long long*>(p.positions)[where];
-    double turns = pos * (p.freqs[pair] * 0.15915494309189533577);  // 1 / 2 pi
-    turns -= rint(turns);
+    const int t = i / p.half, pair = i - t * p.half;
+    double whole = pos[t] * (p.freqs[pair] * 0.15915494309189533577);  // turns: 1 / 2 pi
+    whole -= rint(whole);
     float sn, cs;
-    sincospif((float)(2.0 * turns), &sn, &cs);
+    sincospif((float)(2.0 * whole), &sn, &cs);
     turn[i] = make_float2(p.scale * cs, p.sign * (p.scale * sn));
   }
   __syncthreads();
-  while (i0 < all) {
+  while (row < rows) {
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k)
-      if (i0 + k * THREADS < all) finish(at[k], u[k]);
-    i0 += UNROLL * THREADS;
-    load_all();
+    for (int k = 0; k < UNROLL; ++k) {
+      if (row + k * lanes >= rows) break;
+      if (!turns) {
+        *reinterpret_cast<Raw*>(out[k] + first) = a[k];
+        continue;
+      }
+      float x[V], y[V];
+      Chunk<T, V>::unpack(a[k], x);
+      if (TWO) Chunk<T, V>::unpack(b[TWO ? k : 0], y);
+      const float2* cs = turn + of[k] * p.half + PAIRS * unit;
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        const float2 c = cs[e];
+        float& u = TWO ? x[e % V] : x[(2 * e) % V];
+        float& v = TWO ? y[e % V] : x[(2 * e + 1) % V];
+        const float r = u * c.x - v * c.y;
+        v = v * c.x + u * c.y;
+        u = r;
+      }
+      store_vec<T, V>(out[k], first, x);
+      if (TWO) store_vec<T, V>(out[k], second, y);
+    }
+    row += UNROLL * lanes;
+    if (row >= rows && unit + wide < p.units) {  // (heads of more chunks than the CTA has threads)
+      unit += wide;
+      row = lane;
+      tok = lane / p.heads;
+      head = lane - tok * p.heads;
+      begin_unit();
+    }
+    load();
   }
 }
 
 template <typename T>
-static cudaError_t launch(const Params& p, bool vec, unsigned grid, cudaStream_t st) {
+static cudaError_t launch(const Params& p, bool vec, bool half, unsigned grid, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
   host_count_launch();
-  if (vec) rotate<T, 16 / sizeof(T)><<<grid, THREADS, 0, st>>>(p);
-  else rotate<T, 1><<<grid, THREADS, 0, st>>>(p);
+  if (vec) half ? rotate<T, V, true><<<grid, THREADS, 0, st>>>(p) : rotate<T, V, false><<<grid, THREADS, 0, st>>>(p);
+  else half ? rotate<T, 1, true><<<grid, THREADS, 0, st>>>(p) : rotate<T, 1, false><<<grid, THREADS, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -172,7 +175,8 @@ extern "C" int amsim_rotary(void* stream, const void* x, void* out, int heads, c
   Params p = {};
   const int per = dtype == 0 ? 4 : 8;
   const bool in_place = (!heads || x == out) && (!heads2 || x2 == out2);
-  bool vec = rotary_dim / 2 % per == 0 && (in_place || (dim - rotary_dim) % per == 0);
+  const bool half = !(flags & AMSIM_ROTARY_INTERLEAVED);
+  bool vec = (half ? rotary_dim / 2 : rotary_dim) % per == 0 && (in_place || (dim - rotary_dim) % per == 0);
   p.side[0] = {x, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5]};
   p.side[1] = {x2, out2, strides[6], strides[7], strides[8], strides[9], strides[10], strides[11]};
   for (int i = 0; i < 2; ++i) {
@@ -187,24 +191,24 @@ extern "C" int amsim_rotary(void* stream, const void* x, void* out, int heads, c
   const int v = vec ? per : 1;
   p.positions = positions; p.freqs = freqs;
   p.pos_b = strides[12]; p.pos_s = strides[13];
-  p.tokens = batch * seq;
-  p.half = rotary_dim / 2; p.rot = rotary_dim; p.n_rot = p.half / v;
-  const uint32_t units = p.n_rot + (in_place ? 0 : (dim - rotary_dim) / v);
-  p.seq = make_div((uint32_t)seq); p.units = make_div(units); p.heads = make_div((uint32_t)(heads + heads2));
-  p.heads0 = heads;
-  p.interleaved = (flags & AMSIM_ROTARY_INTERLEAVED) != 0; p.pos32 = (flags & AMSIM_ROTARY_POS32) != 0;
+  p.tokens = batch * seq; p.seq = seq;
+  p.heads = heads + heads2; p.heads0 = heads;
+  p.half = rotary_dim / 2; p.rot = rotary_dim;
+  p.n_rot = half || v == 1 ? p.half / v : rotary_dim / v;
+  p.units = p.n_rot + (in_place ? 0 : (dim - rotary_dim) / v);
+  p.pos32 = (flags & AMSIM_ROTARY_POS32) != 0;
   p.scale = scale; p.sign = flags & AMSIM_ROTARY_INVERSE ? -1.f : 1.f;
-  // Tokens of a CTA: two rounds of units for every thread, as long as that leaves four CTAs a multiprocessor; their angles fit the table.
-  const long long per_token = (long long)units * (heads + heads2);
-  long long n = 2 * UNROLL * THREADS / per_token;
+  // Tokens of a CTA: 16 heads for every thread, as long as that leaves four CTAs a multiprocessor; their angles fit the table.
+  const long long per_token = (long long)p.units * p.heads;
+  long long n = 16 * THREADS / per_token;
   n = n < MAX_PAIRS / p.half ? n : MAX_PAIRS / p.half;
+  n = n < MAX_TOKENS ? n : MAX_TOKENS;
   const long long spread = p.tokens / (4LL * host_sm_count(host_device()));
   n = n < spread ? n : spread;
   p.tokens_per_cta = (int)(n < 1 ? 1 : n);
-  if (per_token >= (1ll << 31)) return host_fail(AMSIM_ERR_UNSUPPORTED, "rotary: more than 2^31 pieces in a token");
   const long long ctas = (p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
   if (ctas >= (1ll << 31)) return host_fail(AMSIM_ERR_UNSUPPORTED, "rotary: more than 2^31 tokens");
   cudaStream_t st = (cudaStream_t)stream;
-  AMSIM_HOST_TRY(dtype == 0 ? launch<float>(p, vec, (unsigned)ctas, st) : dtype == 1 ? launch<__nv_bfloat16>(p, vec, (unsigned)ctas, st) : launch<__half>(p, vec, (unsigned)ctas, st));
+  AMSIM_HOST_TRY(dtype == 0 ? launch<float>(p, vec, half, (unsigned)ctas, st) : dtype == 1 ? launch<__nv_bfloat16>(p, vec, half, (unsigned)ctas, st) : launch<__half>(p, vec, half, (unsigned)ctas, st));
   return AMSIM_OK;
 }
