@@ -33,7 +33,7 @@ EXPORTS = [
     "amsim_debug_fastdiv", "amsim_debug_launch_count", "amsim_debug_reload_env", "amsim_debug_bounds_report",
     "amsim_async_status", "amsim_debug_wait_report",
     "amsim_residual_norm", "amsim_residual_norm_grad_workspace", "amsim_residual_norm_grad",
-    "amsim_rotary", "amsim_adamw", "amsim_mx_bytes", "amsim_mx_quantize", "amsim_mx_dequantize", "amsim_mx_matmul",
+    "amsim_rotary", "amsim_adamw", "amsim_mx_bytes", "amsim_mx_quantize_workspace", "amsim_mx_quantize", "amsim_mx_dequantize", "amsim_mx_matmul",
 ]
 
 
@@ -98,7 +98,9 @@ def _load() -> C.CDLL:
     L.amsim_adamw.argtypes = [vp, ip] + [vp] * 9 + [d, vp, d, d, d, d, vp, u, ip, ip, ip]
     L.amsim_mx_bytes.argtypes = [ll, ll]
     L.amsim_mx_bytes.restype = sz
-    L.amsim_mx_quantize.argtypes = [vp, vp, ll, ll, ip, vp, vp]
+    L.amsim_mx_quantize_workspace.argtypes = [ll, ll]
+    L.amsim_mx_quantize_workspace.restype = sz
+    L.amsim_mx_quantize.argtypes = [vp, vp, ll, ll, ip, vp, vp, vp, vp, sz]
     L.amsim_mx_dequantize.argtypes = [vp, vp, ll, ll, ip, vp, ip]
     L.amsim_mx_matmul.argtypes = [vp, vp, vp, ll, ll, ll, vp, ip, vp, ip]
     return L

@@ -6,7 +6,9 @@
 // any alignment, one bias value a thread.
 //
 // Large products: two CTAs (tcgen05 cta_group::2) share a tile of 256 output columns x 256 tokens; each loads 128 rows of either
-// operand, the tensor cores read both halves.  Small ones: one CTA and a tile of 128 columns x up to 128 tokens.  A warp issues bulk copies, one
+// operand, the tensor cores read both halves.  Small ones: one CTA and a tile of 128 columns x up to 128 tokens; where those
+// leave multiprocessors idle, 2, 4 or 8 CTAs (a cluster) take a share of the reduction each, put their sums in shared memory and
+// each finishes a share of the tokens, adding the others' sums in their order through distributed shared memory.  A warp issues bulk copies, one
 // more the products, the rest take finished tiles out of tensor memory into registers and write them while the next
 // tile's products run.
 //
@@ -32,6 +34,7 @@ struct GemmParams {
   int last_steps;             // 64-element steps of the last tile along the reduction
   int chunk;                  // tiles summed in tensor memory at a time
   int relu, no_tries;
+  int split;                  // CTAs of a cluster that share a tile's reduction (one CTA a tile otherwise)
   int tiles_n, tiles;         // output tiles along the columns, in all
   unsigned* stuck;
 };
@@ -170,7 +173,9 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
   const uint32_t smem0 = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int lane = threadIdx.x & 31, w = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const uint32_t rank = CG == 2 ? blockIdx.x & 1u : 0u;
-  const int team = blockIdx.x / CG, teams = gridDim.x / CG;
+  const int split = CG == 1 ? p.split : 1, share = split > 1 ? blockIdx.x % split : 0;
+  const int team = blockIdx.x / (CG * split), teams = gridDim.x / (CG * split);
+  const int k_begin = (int)((long long)p.kt * share / split), k_end = (int)((long long)p.kt * (share + 1) / split);
   const uint32_t bar_full = smem_addr(bars), bar_empty = bar_full + 8 * S::STAGES, bar_peer = bar_empty + 8 * S::STAGES;
   const uint32_t bar_done = bar_peer + 8 * S::STAGES, bar_free = bar_done + 8 * S::NACC, bar_exit = bar_free + 8 * S::NACC;
   if (threadIdx.x == 0) {
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
       const uint8_t* src_s[S::HALVES];
 #pragma unroll
       for (int h = 0; h < S::HALVES; ++h) src_s[h] = p.a + (long long)min(tt * CG + h, p.a_tiles - 1) * p.kt * TILE_BYTES + CODE_BYTES;
-      for (int k = 0; k < p.kt; ++k) {
+      for (int k = k_begin; k < k_end; ++k) {
         wt.wait_warp(bar_empty + 8 * b, phase);
         if (lane == 0 && !wt.dead) {
           const uint32_t at = smem0 + b * S::STAGE, bar = bar_full + 8 * b;
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
     const uint32_t lead = cluster_addr(bar_peer, 0), word = cluster_addr(smem_addr(&signal), 0);
     uint32_t b = 0, phase = 0;
     for (int tile = team; tile < p.tiles; tile += teams)
-      for (int k = 0; k < p.kt; ++k) {
+      for (int k = k_begin; k < k_end; ++k) {
         wt.wait_warp(bar_full + 8 * b, phase);
         if (lane == 0 && !wt.dead) st_async(word, 0, lead + 8 * b);
         if (++b == S::STAGES) b = 0, phase ^= 1;
@@ -248,10 +253,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
     constexpr uint32_t id0 = idesc(128 * CG, BN);
     for (int tile = team; tile < p.tiles; tile += teams) {
       int left = 0;
-      for (int k = 0; k < p.kt; ++k) {
+      for (int k = k_begin; k < k_end; ++k) {
         const bool first = left == 0;
         if (first) {
-          left = min(p.chunk, p.kt - k);
+          left = min(p.chunk, k_end - k);
           wt.wait_warp(bar_free + 8 * acc, acc_phase);
         }
         if (CG == 2 && lane == 0 && !wt.dead) mbar_expect(bar_peer + 8 * b, 4);
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
       }
       end_chunk();
 #pragma unroll 1
-      for (int k = p.chunk; k < p.kt; k += p.chunk) {
+      for (int k = k_begin + p.chunk; k < k_end; k += p.chunk) {
         begin_chunk();
 #pragma unroll
         for (int c = 0; c < S::COLS; c += 16) {
@@ -337,17 +342,53 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
       }
       const long long n = (long long)(tn * CG + (int)rank) * 128 + quarter * 32 + lane;
       const long long t0 = (long long)tt * BN + part * S::COLS;
-      if (n < p.n) {
-        const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
-        T* out = static_cast<T*>(p.out) + t0 * p.n + n;
-        const int count = (int)min((long long)S::COLS, p.m - t0);
-        const long long pitch = p.n;
-        auto write = [&](float o) {
-          if (p.bias) o += bias;
-          *out = elem_from_float<T>(p.relu && o < 0.f ? 0.f : o);
-          out += pitch;
-          asm volatile("" : "+l"(out));  // (one running address: the compiler would keep one for every column, and spill)
-        };
+      const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.f;
+      const long long pitch = p.n;
+      T* out = static_cast<T*>(p.out) + t0 * p.n + n;
+      auto write = [&](float o) {
+        if (p.bias) o += bias;
+        *out = elem_from_float<T>(p.relu && o < 0.f ? 0.f : o);
+        out += pitch;
+        asm volatile("" : "+l"(out));  // (one running address: the compiler would keep one for every column, and spill)
+      };
+      const int count = (int)min((long long)S::COLS, p.m - t0);
+      if (CG == 1 && split > 1) {  // (one tile a cluster, and its stages are all used up: their place takes the sums)
+        const uint32_t mine = smem0 + (quarter * 32 + lane) * 16;  // four columns at a time, 2 KB apart
+#pragma unroll
+        for (int c = 0; c < S::COLS; c += 4)
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + c * 512), "f"(v[c]), "f"(v[c + 1]), "f"(v[c + 2]), "f"(v[c + 3]) : "memory");
+        cluster_barrier();
+        const int c0 = S::COLS / split * share, c1 = min(count, S::COLS / split * (share + 1));  // (S::COLS / split is a multiple of 4)
+        out += c0 * pitch;
+        constexpr int AT_ONCE = S::COLS < 64 ? 8 : 32;  // columns of two CTAs on their way before the first is added: each round waits for the other CTA's memory
+#pragma unroll 1
+        for (int c = c0; c < c1; c += AT_ONCE) {
+          float sum[AT_ONCE];
+#pragma unroll
+          for (int j = 0; j < AT_ONCE; ++j) sum[j] = 0.f;
+#pragma unroll 1
+          for (int i = 0; i < split; i += 2) {  // (split is even)
+            float x[2][AT_ONCE];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t from = cluster_addr(mine, i + h) + c * 512;
+#pragma unroll
+              for (int j = 0; j < AT_ONCE; j += 4)
+                if (c + j < c1) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[h][j]), "=f"(x[h][j + 1]), "=f"(x[h][j + 2]), "=f"(x[h][j + 3]) : "r"(from + j * 512) : "memory");
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < AT_ONCE; ++j)
+                if (c + j < c1) sum[j] = __fadd_rn(sum[j], x[h][j]);
+          }
+          if (n < p.n) {
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+              if (c + j < c1) write(sum[j]);
+          }
+        }
+      } else if (n < p.n) {
         if (count == S::COLS) {
 #pragma unroll
           for (int c = 0; c < S::COLS; ++c) write(v[c]);
@@ -366,9 +407,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1) gemm(const __grid_c
     last.wait_warp(bar_exit, 0);
     if (wt.dead) __nanosleep(100000);
   }
+  if (CG == 1 && split > 1 && w < 4) cluster_barrier();  // (the one that the sums wait at)
   fence_before();
   __syncthreads();
-  if (CG == 2) cluster_barrier();
+  if (CG == 2 || split > 1) cluster_barrier();  // neither leaves while another may still reach its memory
   if (w == 1) tmem_free<CG>(tmem);
 }
 

@@ -498,15 +498,15 @@ class _MXDenseFn(torch.autograd.Function):
         x_shape, w_shape, x_type, w_type = ctx.cfg
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         g = (torch.ops.aten.threshold_backward(g, y, 0.0) if y is not None else g).contiguous()
+        db = torch.empty(g.shape[1], dtype=torch.float32, device=g.device) if want_b else None
         if want_x and want_w:
-            g_rows, g_cols = ops.mx_quantize_both(g)
+            g_rows, g_cols = ops.mx_quantize_both(g, sums=db)
         else:
+            if want_b:
+                torch.sum(g, 0, dtype=torch.float32, out=db)
             g_rows, g_cols = (ops.mx_quantize(g) if want_x else None), (ops.mx_quantize(g, axis=0) if want_w else None)
         dx = ops.mx_matmul(g_rows, ops.MXTensor(w_data, w_shape, 1), out_dtype=x_type) if want_x else None
         dw = ops.mx_matmul(ops.MXTensor(x_data, x_shape, 0), g_cols, out_dtype=w_type) if want_w else None
-        db = None
-        if want_b:
-            db = ops.bias_grad(g) if g.dtype == torch.float32 else g.sum(0, dtype=torch.float32)
         return dx, dw, db, None
 
 

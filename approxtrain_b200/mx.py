@@ -55,13 +55,15 @@ def _matrix(x):
     return x.contiguous()
 
 
-def _quantize(x, along: bool, across: bool):
+def _quantize(x, along: bool, across: bool, sums=None):
     rows, cols = x.shape
     one = torch.empty(lib.amsim_mx_bytes(rows, cols), dtype=torch.uint8, device=x.device) if along else None
     two = torch.empty(lib.amsim_mx_bytes(cols, rows), dtype=torch.uint8, device=x.device) if across else None
+    size = lib.amsim_mx_quantize_workspace(rows, cols) if sums is not None else 0
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     if (along and rows) or (across and cols):
-        _call(x.device, lib.amsim_mx_quantize, x.data_ptr(), rows, cols, _TYPES[x.dtype], one.data_ptr() if along and rows else None,
-              two.data_ptr() if across and cols else None)
+        _call(x.device, lib.amsim_mx_quantize, x.data_ptr(), rows, cols, _TYPES[x.dtype], one.data_ptr() if along else None,
+              two.data_ptr() if across else None, sums.data_ptr() if sums is not None else None, ws.data_ptr() if size else None, size)
     return (MXTensor(one, (rows, cols), 1) if along else None), (MXTensor(two, (rows, cols), 0) if across else None)
 
 
@@ -76,9 +78,14 @@ def mx_quantize(x: torch.Tensor, axis: int = -1) -> MXTensor:
     return _quantize(x, along, not along)[0 if along else 1]
 
 
-def mx_quantize_both(x: torch.Tensor):
-    """``(mx_quantize(x, 1), mx_quantize(x, 0))`` with one read of x."""
-    return _quantize(_matrix(x), True, True)
+def mx_quantize_both(x: torch.Tensor, sums: torch.Tensor = None):
+    """``(mx_quantize(x, 1), mx_quantize(x, 0))`` with one read of x.  ``sums`` (float32 [columns], optional): receives the sums of
+    x's columns from the same read, FP32 in a fixed order (the bias gradient, where x is an output's gradient)."""
+    x = _matrix(x)
+    if sums is not None and (not isinstance(sums, torch.Tensor) or sums.dtype != torch.float32 or tuple(sums.shape) != (x.shape[1],) or sums.device != x.device
+                             or not sums.is_contiguous()):
+        raise ValueError(f"sums must be contiguous float32 of shape [{x.shape[1]}] on {x.device}")
+    return _quantize(x, True, True, sums)
 
 
 def mx_matmul(a: MXTensor, b: MXTensor, bias=None, activation=None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:

@@ -367,10 +367,13 @@ int amsim_adamw(void* stream, int tensors, const void* const* params, const void
  * Quantise: x (rows x cols, dense) along its columns' axis into `along` (rows x cols) and / or along its rows' axis into
  * `across` (cols x rows, k = rows); either may be NULL, both take one read of x.  Scale of a block: the power of two that puts its
  * largest element in [4, 8); elements are rounded to nearest, ties to even, beyond 6 to 6.  An infinity or NaN makes its
- * block NaN.  Dequantise: `transposed` writes k x rows (a matrix quantised across, as it was). */
+ * block NaN.  `sums` (cols floats, may be NULL, with `across`): the sums of x's columns, FP32 in a fixed order (a bias gradient
+ * from the read that the codes need anyway); takes amsim_mx_quantize_workspace bytes of device scratch.  Dequantise: `transposed` writes k x rows (a matrix quantised across, as it was). */
 size_t amsim_mx_bytes(long long rows, long long k);
+size_t amsim_mx_quantize_workspace(long long rows, long long cols);
 int amsim_mx_quantize(void* stream, const void* x, long long rows, long long cols, int dtype,
-                      void* along, void* across);
+                      void* along, void* across, float* sums, void* workspace,
+                      size_t workspace_bytes);
 int amsim_mx_dequantize(void* stream, const void* data, long long rows, long long k,
                         int transposed, void* out, int dtype);
 /* out[i][j] = act(sum over k of a[i][k] b[j][k] + bias[j]), out m x n dense of `dtype`; bias (n floats) may be NULL.  Products are

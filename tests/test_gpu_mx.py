@@ -107,7 +107,8 @@ def _product(a, b, bias, relu, out_dtype):
 
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 32), (3, 5, 64), (16, 100, 65), (17, 300, 256), (32, 129, 300), (33, 64, 512), (64, 1000, 100), (65, 128, 257), (100, 300, 700),
-                                   (128, 128, 4096), (129, 257, 520), (200, 2000, 96), (1, 8000, 512), (16, 8000, 512)])
+                                   (128, 128, 4096), (129, 257, 520), (200, 2000, 96), (1, 8000, 512), (16, 8000, 512),
+                                   (16, 128, 8192), (5, 2048, 4200), (64, 300, 9000), (128, 200, 17000), (40, 128, 17000), (512, 2048, 8192), (100, 1000, 1500)])
 def test_small_products(out_dtype, m, n, k):
     a, b = _rand(m, k, seed=m), _rand(n, k, seed=n + 1, spread=0.5)
     _product(a, b, None, False, out_dtype)
@@ -145,6 +146,20 @@ def test_empty_sizes():
         assert torch.equal(ops.mx_matmul(q(3, 0), q(n, 0), bias=bias), bias.expand(3, n))
     a, b = ops.mx_quantize_both(torch.zeros(0, 9, device="cuda"))
     assert a.dequantize().shape == (0, 9) and b.dequantize().shape == (0, 9)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(0, 5), (1, 1), (3, 200), (128, 128), (129, 33), (5000, 300), (2049, 1000)])
+def test_column_sums(t, shape):
+    from approxtrain_b200 import ops
+    x = _rand(*shape, t=t)
+    sums = torch.full((shape[1],), float("nan"), device="cuda")
+    a, b = ops.mx_quantize_both(x, sums=sums)
+    # 8 terms a chain, then at most 2 + 2 + rows / 2048 + 16 partial sums
+    tol = (8 + 4 + shape[0] / 2048 + 16) * 2.0 ** -24 * x.double().abs().sum(0)
+    assert bool(((sums.double() - x.double().sum(0)).abs() <= tol).all())
+    if shape[0]:
+        assert _same(a.dequantize(), _values(x, 1)) and _same(b.dequantize(), _values(x, 0))
 
 
 def test_transposed_operands_and_repeats():

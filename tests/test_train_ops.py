@@ -153,7 +153,12 @@ def test_mx_refusals(L):
     with pytest.raises(ValueError, match="CUDA"):
         ops.mx_quantize(torch.zeros(2, 4))
     p = 1 << 20
-    q, d, m = L.lib.amsim_mx_quantize, L.lib.amsim_mx_dequantize, L.lib.amsim_mx_matmul
+    d, m = L.lib.amsim_mx_dequantize, L.lib.amsim_mx_matmul
+
+    def q(stream, x, rows, cols, dtype, along, across, sums=None, ws=None, size=0):
+        return L.lib.amsim_mx_quantize(stream, x, rows, cols, dtype, along, across, sums, ws, size)
+    assert q(None, p, 4, 4, 0, p, None, sums=p, ws=p, size=1 << 20) == L.ERR_INVALID
+    assert q(None, p, 4, 4, 0, p, p, sums=p) == L.ERR_WORKSPACE and q(None, p, 4, 4, 0, p, p, sums=p, ws=p, size=8) == L.ERR_WORKSPACE
     assert L.lib.amsim_mx_bytes(1, 1) == 17408 and L.lib.amsim_mx_bytes(129, 257) == 4 * 17408 and L.lib.amsim_mx_bytes(0, 5) == 0 and L.lib.amsim_mx_bytes(5, 0) == 17408
     assert q(None, p, -1, 4, 0, p, None) == L.ERR_INVALID and q(None, p, 4, 4, 3, p, None) == L.ERR_INVALID
     assert q(None, p, 4, 4, 0, None, None) == L.ERR_INVALID and q(None, None, 4, 4, 0, p, None) == L.ERR_INVALID
