@@ -175,75 +175,129 @@ __device__ __forceinline__ float2 unpack8(uint16_t v) {
   return __half22float2(h2);
 }
 
-// A block of 8-bit moments as a warp has loaded it: 8 elements a lane, four adjacent ones twice (VEC), or lane after lane.
+// Two FP32 operations in one instruction (each rounded as if alone).
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(a), "f"(b));
+  return t;
+}
+__device__ __forceinline__ void apart(Two t, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v)); }
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two t;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+// (the sums apart: as one instruction they ended up fused with the products, and single codes differed)
+__device__ __forceinline__ void sum_apart(Two a, Two b, float& x, float& y) {
+  float a0, a1, b0, b1;
+  apart(a, a0, a1);
+  apart(b, b0, b1);
+  x = __fadd_rn(a0, b0);
+  y = __fadd_rn(a1, b1);
+}
+
+// Where a lane's elements of a block are: four adjacent ones twice, 128 apart (vec), or one every 32.  The addresses walk from
+// block to block; computed anew for each they were a fifth of the instructions.
+struct Cursor {
+  char *p, *m, *v;
+  const char* g;
+  long long left;       // elements of the tensor from this block on
+  uint32_t place;       // of the block among the moments, folded to 32 bits (a block does not straddle 2^32)
+  uint32_t scale;       // number of its scales: places are below 2^40
+  float keep;           // 1 - lr decay
+  bool vec;
+};
 struct Block {
   float p[8], g[8], ms, vs;
   uint32_t mc[2], vc[2];
 };
-template <bool VEC>
-__device__ __forceinline__ int elem_of(int j) {
+
+// The low and high words of a block's place, as one.
+__device__ __forceinline__ uint32_t fold(uint32_t block) { return block * BLOCK + (block >> 24) * 0x9E3779B1u; }
+
+template <typename TP, typename TG>
+__device__ __forceinline__ void point(Cursor& at, const Entry& e, const Common& c, long long base, float lr) {
   const int lane = threadIdx.x & 31;
-  return VEC ? (j >> 2) * 128 + 4 * lane + (j & 3) : j * 32 + lane;
+  at.vec = ((((uintptr_t)e.p) | ((uintptr_t)e.g)) & 15) == 0;
+  const int mine = at.vec ? 4 * lane : lane;
+  const unsigned long long place = (unsigned long long)(e.at + base);
+  at.p = static_cast<char*>(e.p) + (base + mine) * sizeof(TP);
+  at.g = static_cast<const char*>(e.g) + (base + mine) * sizeof(TG);
+  at.m = static_cast<char*>(c.m) + place + mine;
+  at.v = static_cast<char*>(c.v) + place + mine;
+  at.left = e.n - base;
+  at.scale = (uint32_t)(place / BLOCK);
+  at.place = fold(at.scale);
+  at.keep = 1.f - lr * e.decay;
+}
+template <typename TP, typename TG>
+__device__ __forceinline__ void walk(Cursor& at, int blocks) {
+  at.p += blocks * BLOCK * sizeof(TP);
+  at.g += blocks * BLOCK * sizeof(TG);
+  at.m += blocks * BLOCK;
+  at.v += blocks * BLOCK;
+  at.left -= blocks * BLOCK;
+  at.scale += blocks;
+  at.place = fold(at.scale);
 }
 
+// Element number j of a lane: its distance from the lane's first one.
+template <bool VEC>
+__device__ __forceinline__ constexpr int elem_of(int j) { return VEC ? (j >> 2) * 128 + (j & 3) : j * 32; }
+
 template <typename TP, typename TG, bool VEC>
-__device__ __forceinline__ void load8(Block& b, const Entry& e, const Common& c, long long base) {
-  const long long place = e.at + base;
-  const uint8_t* const m8 = static_cast<const uint8_t*>(c.m) + place;
-  const uint8_t* const v8 = static_cast<const uint8_t*>(c.v) + place;
-  const int n = (int)(e.n - base < BLOCK ? e.n - base : BLOCK);
-  b.ms = c.m_scale[place / BLOCK];
-  b.vs = c.v_scale[place / BLOCK];
+__device__ __forceinline__ void load8(Block& b, const Cursor& at, const Common& c) {
+  const int lane = threadIdx.x & 31, n = at.left < BLOCK ? (int)at.left - (VEC ? 4 * lane : lane) : BLOCK;  // (elements from the lane's first on)
+  b.ms = c.m_scale[at.scale];
+  b.vs = c.v_scale[at.scale];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (VEC) {
-      b.mc[h] = *reinterpret_cast<const uint32_t*>(m8 + elem_of<VEC>(4 * h));
-      b.vc[h] = *reinterpret_cast<const uint32_t*>(v8 + elem_of<VEC>(4 * h));
+      b.mc[h] = *reinterpret_cast<const uint32_t*>(at.m + elem_of<VEC>(4 * h));
+      b.vc[h] = *reinterpret_cast<const uint32_t*>(at.v + elem_of<VEC>(4 * h));
     } else {
       b.mc[h] = b.vc[h] = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        b.mc[h] |= (uint32_t)m8[elem_of<VEC>(4 * h + i)] << (8 * i);
-        b.vc[h] |= (uint32_t)v8[elem_of<VEC>(4 * h + i)] << (8 * i);
+        b.mc[h] |= (uint32_t)(uint8_t)at.m[elem_of<VEC>(4 * h + i)] << (8 * i);
+        b.vc[h] |= (uint32_t)(uint8_t)at.v[elem_of<VEC>(4 * h + i)] << (8 * i);
       }
     }
     if (VEC && n == BLOCK) {
-      float t[4];
-      load_vec<TP, 4>(e.p, base + elem_of<VEC>(4 * h), t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b.p[4 * h + i] = t[i];
-      load_vec<TG, 4>(e.g, base + elem_of<VEC>(4 * h), t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b.g[4 * h + i] = t[i];
+      load_vec<TP, 4>(at.p, elem_of<VEC>(4 * h), *reinterpret_cast<float(*)[4]>(b.p + 4 * h));
+      load_vec<TG, 4>(at.g, elem_of<VEC>(4 * h), *reinterpret_cast<float(*)[4]>(b.g + 4 * h));
     } else {
 #pragma unroll
       for (int j = 4 * h; j < 4 * h + 4; ++j) {
-        const bool ok = elem_of<VEC>(j) < n;
-        b.p[j] = ok ? load1<TP>(e.p, base + elem_of<VEC>(j)) : 0.f;
-        b.g[j] = ok ? load1<TG>(e.g, base + elem_of<VEC>(j)) : 0.f;
+        const bool ok = n == BLOCK || elem_of<VEC>(j) < n;
+        b.p[j] = ok ? load1<TP>(at.p, elem_of<VEC>(j)) : 0.f;
+        b.g[j] = ok ? load1<TG>(at.g, elem_of<VEC>(j)) : 0.f;
       }
     }
   }
 }
 
 template <typename TP, bool VEC>
-__device__ __forceinline__ void step8(const Block& in, const Entry& e, const Common& c, long long base, const Rates& r) {
-  const long long place = e.at + base;
-  const int n = (int)(e.n - base < BLOCK ? e.n - base : BLOCK);
-  const float keep = 1.f - r.lr * e.decay;
+__device__ __forceinline__ void step8(const Block& in, const Cursor& at, const Common& c, const Rates& r) {
+  const int lane = threadIdx.x & 31, n = at.left < BLOCK ? (int)at.left - (VEC ? 4 * lane : lane) : BLOCK;
+  const Two b1 = two(r.b1, r.b1), c1 = two(r.c1, r.c1), b2 = two(r.b2, r.b2), c2 = two(r.c2, r.c2), gs = two(r.g_scale, r.g_scale), ms = two(in.ms, in.ms), vs = two(in.vs, in.vs);
   float p[8], m[8], root[8];
   uint32_t m_top = 0, v_top = 0;
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     const float2 mv = unpack8((uint16_t)(in.mc[j >> 2] >> (8 * (j & 3)))), vv = unpack8((uint16_t)(in.vc[j >> 2] >> (8 * (j & 3))));
+    // (as in moments(), two at a time)
+    const Two g = mul(two(in.g[j], in.g[j + 1]), gs), old = mul(two(vv.x, vv.y), vs);
+    float v[2];
+    sum_apart(mul(b1, mul(two(mv.x, mv.y), ms)), mul(c1, g), m[j], m[j + 1]);
+    sum_apart(mul(b2, mul(old, old)), mul(c2, mul(g, g)), v[0], v[1]);
 #pragma unroll
     for (int i = j; i < j + 2; ++i) {
-      m[i] = __fmul_rn(i == j ? mv.x : mv.y, in.ms);
-      const float old = __fmul_rn(i == j ? vv.x : vv.y, in.vs);
-      float v = __fmul_rn(old, old);
-      moments(in.g[i], m[i], v, r);
-      root[i] = sqrtf(v);
-      p[i] = update(in.p[i], m[i], root[i], keep, r);
+      root[i] = sqrtf(v[i - j]);
+      p[i] = update(in.p[i], m[i], root[i], at.keep, r);
       m_top = max(m_top, __float_as_uint(m[i]) & 0x7FFFFFFFu);
       v_top = max(v_top, __float_as_uint(root[i]));
     }
@@ -251,41 +305,38 @@ __device__ __forceinline__ void step8(const Block& in, const Entry& e, const Com
   const float mt = __uint_as_float(__reduce_max_sync(0xffffffffu, m_top)), vt = __uint_as_float(__reduce_max_sync(0xffffffffu, v_top));
   // (the scale as a product with 1 / 448 and its inverse as 448 times a reciprocal, each rounded)
   const float m_inv = mt >= 0x1p-100f ? __fmul_rn(448.f, __frcp_rn(mt)) : 0.f, v_inv = vt >= 0x1p-100f ? __fmul_rn(448.f, __frcp_rn(vt)) : 0.f;
-  const uint32_t place32 = (uint32_t)place + (uint32_t)((unsigned long long)place >> 32) * 0x9E3779B1u;  // (a block does not straddle 2^32)
-  uint8_t* const m8 = static_cast<uint8_t*>(c.m) + place;
-  uint8_t* const v8 = static_cast<uint8_t*>(c.v) + place;
+  const uint32_t place = at.place + (VEC ? 4 * lane : lane);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t a[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int j = 4 * h + i;
-      const uint32_t rnd = mix((place32 + elem_of<VEC>(j)) ^ r.key);
+      const uint32_t rnd = mix((place + elem_of<VEC>(j)) ^ r.key);
       a[i] = (round8(m[j], m_inv, ((rnd << 4) & 0xFFFF0u) | 8u, false) & 0x7FFFFFFFu) | (__float_as_uint(m[j]) & 0x80000000u);
       b[i] = round8(root[j], v_inv, ((rnd >> 12) & 0xFFFF0u) | 8u, true);
     }
     if (VEC) {
-      *reinterpret_cast<uint32_t*>(m8 + elem_of<VEC>(4 * h)) = __byte_perm(__byte_perm(a[0], a[1], 0x0073), __byte_perm(a[2], a[3], 0x0073), 0x5410);
-      *reinterpret_cast<uint32_t*>(v8 + elem_of<VEC>(4 * h)) = __byte_perm(__byte_perm(b[0], b[1], 0x0073), __byte_perm(b[2], b[3], 0x0073), 0x5410);
+      *reinterpret_cast<uint32_t*>(at.m + elem_of<VEC>(4 * h)) = __byte_perm(__byte_perm(a[0], a[1], 0x0073), __byte_perm(a[2], a[3], 0x0073), 0x5410);
+      *reinterpret_cast<uint32_t*>(at.v + elem_of<VEC>(4 * h)) = __byte_perm(__byte_perm(b[0], b[1], 0x0073), __byte_perm(b[2], b[3], 0x0073), 0x5410);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        m8[elem_of<VEC>(4 * h + i)] = (uint8_t)(a[i] >> 24);
-        v8[elem_of<VEC>(4 * h + i)] = (uint8_t)(b[i] >> 24);
+        at.m[elem_of<VEC>(4 * h + i)] = (char)(a[i] >> 24);
+        at.v[elem_of<VEC>(4 * h + i)] = (char)(b[i] >> 24);
       }
     }
     if (VEC && n == BLOCK) {
-      const float t[4] = {p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]};
-      store_vec<TP, 4>(e.p, base + elem_of<VEC>(4 * h), t);
+      store_vec<TP, 4>(at.p, elem_of<VEC>(4 * h), *reinterpret_cast<float(*)[4]>(p + 4 * h));
     } else {
 #pragma unroll
       for (int j = 4 * h; j < 4 * h + 4; ++j)
-        if (elem_of<VEC>(j) < n) store1<TP>(e.p, base + elem_of<VEC>(j), p[j]);
+        if (n == BLOCK || elem_of<VEC>(j) < n) store1<TP>(at.p, elem_of<VEC>(j), p[j]);
     }
   }
-  if ((threadIdx.x & 31) == 0) {
-    c.m_scale[place / BLOCK] = mt < 0x1p-100f ? 0.f : __fmul_rn(mt, 1.f / 448.f);  // (not a number: neither are the block's moments)
-    c.v_scale[place / BLOCK] = vt < 0x1p-100f ? 0.f : __fmul_rn(vt, 1.f / 448.f);
+  if (lane == 0) {
+    c.m_scale[at.scale] = mt < 0x1p-100f ? 0.f : __fmul_rn(mt, 1.f / 448.f);  // (not a number: neither are the block's moments)
+    c.v_scale[at.scale] = vt < 0x1p-100f ? 0.f : __fmul_rn(vt, 1.f / 448.f);
   }
 }
 
@@ -337,29 +388,38 @@ __global__ void __launch_bounds__(THREADS, BITS == 32 ? 3 : 2) adamw(const __gri
     }
   } else {
     // a CTA's blocks are consecutive, its warps take them in turn, and the next one is on its way while a warp works on one
-    // (without that, 56 million parameters took 258 us instead of 226; what bounds it then is the issue of instructions, about a hundred a parameter)
+    // (without that, 56 million parameters took 258 us instead of 226; what bounds it then is the issue of instructions)
+    constexpr int WARPS = THREADS / 32;
+    __syncthreads();
+    const Rates r = rates;
     const long long begin = c.units * blockIdx.x / gridDim.x, end = c.units * (blockIdx.x + 1) / gridDim.x;
     long long unit = begin + (threadIdx.x >> 5);
     int k = find(tab, unit);
-    auto is_vec = [&](int i) { return ((((uintptr_t)tab.e[i].p) | ((uintptr_t)tab.e[i].g)) & 15) == 0; };
-    auto load = [&](Block& b) {
-      while (k + 1 < c.count && tab.first[k + 1] <= unit) ++k;
-      const long long base = (unit - tab.first[k]) * BLOCK;
-      if (is_vec(k)) load8<TP, TG, true>(b, tab.e[k], c, base);
-      else load8<TP, TG, false>(b, tab.e[k], c, base);
-    };
+    long long next_first = k + 1 < c.count ? tab.first[k + 1] : c.units;  // where the next tensor begins
+    Cursor at;
+    point<TP, TG>(at, tab.e[k], c, (unit - tab.first[k]) * BLOCK, r.lr);
     Block next;
-    if (unit < end) load(next);
-    __syncthreads();
-    const Rates r = rates;
+    auto load = [&]() {
+      if (at.vec) load8<TP, TG, true>(next, at, c);
+      else load8<TP, TG, false>(next, at, c);
+    };
+    if (unit < end) load();
     while (unit < end) {
       const Block now = next;
-      const int at = k;
-      const long long base = (unit - tab.first[at]) * BLOCK;
-      unit += THREADS / 32;
-      if (unit < end) load(next);
-      if (is_vec(at)) step8<TP, true>(now, tab.e[at], c, base, r);
-      else step8<TP, false>(now, tab.e[at], c, base, r);
+      const Cursor here = at;
+      unit += WARPS;
+      if (unit < end) {
+        if (unit < next_first) {
+          walk<TP, TG>(at, WARPS);
+        } else {
+          do ++k; while (k + 1 < c.count && tab.first[k + 1] <= unit);
+          next_first = k + 1 < c.count ? tab.first[k + 1] : c.units;
+          point<TP, TG>(at, tab.e[k], c, (unit - tab.first[k]) * BLOCK, r.lr);
+        }
+        load();
+      }
+      if (here.vec) step8<TP, true>(now, here, c, r);
+      else step8<TP, false>(now, here, c, r);
     }
   }
   if (c.advance && threadIdx.x == 0) {
@@ -436,10 +496,13 @@ extern "C" int amsim_adamw(void* stream, int tensors, const void* const* params,
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0)) return host_fail(AMSIM_ERR_INVALID, "adamw: betas in [0, 1) and eps >= 0 expected");
   if (!step || (tensors && (!params || !grads || !sizes || !decay))) return host_fail(AMSIM_ERR_INVALID, "NULL argument");
   bool any = false;
+  long long all = 0;
   for (int i = 0; i < tensors; ++i) {
     if (sizes[i] < 0 || sizes[i] >= (1ll << 38)) return host_fail(AMSIM_ERR_INVALID, "adamw: tensor %d has %lld elements", i, sizes[i]);
     if (sizes[i] && (!params[i] || !grads[i])) return host_fail(AMSIM_ERR_INVALID, "adamw: NULL tensor %d", i);
     any = any || sizes[i] > 0;
+    all += (sizes[i] + BLOCK - 1) / BLOCK;
+    if (all >= (1ll << 32)) return host_fail(AMSIM_ERR_UNSUPPORTED, "adamw: more than 2^40 elements");
   }
   if (any && (!exp_avg || !exp_avg_sq || (bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)))) return host_fail(AMSIM_ERR_INVALID, "NULL moment pointer");
   if ((((uintptr_t)exp_avg) | ((uintptr_t)exp_avg_sq)) & 15) return host_fail(AMSIM_ERR_INVALID, "adamw: moments must be 16-byte aligned");
