@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/amsim.h"
 
 namespace amsim {
@@ -16,10 +18,22 @@ int host_device();
 int host_stuck_word(int device, unsigned** word);
 int host_report_stuck(int device);
 
+// Lets `kernel` take up to `bytes` of dynamic shared memory: asked for once per device and kernel (`done`: a word of the
+// kernel's own, one bit a device).
+template <typename K>
+cudaError_t host_allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  const int device = host_device();
+  const unsigned long long bit = device >= 0 && device < 64 ? 1ull << device : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 }  // namespace amsim
 
-#define AMSIM_HOST_TRY(expr)                                                                                        \
-  do {                                                                                                              \
-    cudaError_t e_ = (expr);                                                                                        \
-    if (e_ != cudaSuccess) return amsim::host_fail(AMSIM_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
+#define AMSIM_HOST_TRY(...)                                                                                                  \
+  do {                                                                                                                       \
+    cudaError_t e_ = (__VA_ARGS__);                                                                                          \
+    if (e_ != cudaSuccess) return amsim::host_fail(AMSIM_ERR_CUDA, "%s: %s", __func__, cudaGetErrorString(e_)); \
   } while (0)

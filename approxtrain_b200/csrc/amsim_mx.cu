@@ -33,7 +33,7 @@ struct Stage {
 };
 // (back to floats: FP32 in rows of four blocks of 36 words)
 constexpr int Q_BLOCK = 36, Q_ROW = 4 * Q_BLOCK, Q_ROW_T = Q_ROW + 4;
-constexpr int Q_SMEM = 128 * Q_ROW * 4, Q_SMEM_T = 128 * Q_ROW_T * 4;
+constexpr int Q_SMEM_T = 128 * Q_ROW_T * 4;
 
 struct QuantParams {
   const void* x;
@@ -272,14 +272,15 @@ static int check_size(long long rows, long long k, const char* what) {
   return AMSIM_OK;
 }
 
-template <typename K, typename P>
-static cudaError_t launch(K kernel, long long grid, int threads, int smem, int cluster, cudaStream_t st, const P& p) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto kernel, int SMEM, typename P>
+static cudaError_t launch(long long grid, int threads, int cluster, cudaStream_t st, const P& p) {
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = host_allow_smem(kernel, SMEM, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
@@ -304,9 +305,9 @@ static cudaError_t gemm_launch(GemmParams& p, int dtype, int device, cudaStream_
   p.split = 1;
   while (CG == 1 && p.split < 8 && p.tiles * p.split * 2 <= teams && p.kt >= 16 * p.split && S::COLS / p.split >= 8) p.split *= 2;
   if (p.split > 1) grid = (long long)p.tiles * p.split;
-  if (dtype == 0) return launch(gemm<CG, BN, float>, grid, S::THREADS, S::SMEM, CG * p.split, st, p);
-  if (dtype == 1) return launch(gemm<CG, BN, __nv_bfloat16>, grid, S::THREADS, S::SMEM, CG * p.split, st, p);
-  return launch(gemm<CG, BN, __half>, grid, S::THREADS, S::SMEM, CG * p.split, st, p);
+  if (dtype == 0) return launch<gemm<CG, BN, float>, S::SMEM>(grid, S::THREADS, CG * p.split, st, p);
+  if (dtype == 1) return launch<gemm<CG, BN, __nv_bfloat16>, S::SMEM>(grid, S::THREADS, CG * p.split, st, p);
+  return launch<gemm<CG, BN, __half>, S::SMEM>(grid, S::THREADS, CG * p.split, st, p);
 }
 
 }  // namespace mx
@@ -353,8 +354,8 @@ int amsim_mx_quantize(void* stream, const void* x, long long rows, long long col
   const long long grid = p.gx * (across ? 2 * p.across_kt : tiles128(rows));
   if (grid >= (1ll << 31)) return host_fail(AMSIM_ERR_UNSUPPORTED, "mx_quantize: more than 2^31 tiles");
   cudaStream_t st = (cudaStream_t)stream;
-  AMSIM_HOST_TRY(dtype == 0 ? launch(quantise<float>, grid, Q_THREADS, Stage<float>::BYTES, 1, st, p)
-                            : dtype == 1 ? launch(quantise<__nv_bfloat16>, grid, Q_THREADS, Stage<__half>::BYTES, 1, st, p) : launch(quantise<__half>, grid, Q_THREADS, Stage<__half>::BYTES, 1, st, p));
+  AMSIM_HOST_TRY(dtype == 0 ? launch<quantise<float>, Stage<float>::BYTES>(grid, Q_THREADS, 1, st, p)
+                            : dtype == 1 ? launch<quantise<__nv_bfloat16>, Stage<__half>::BYTES>(grid, Q_THREADS, 1, st, p) : launch<quantise<__half>, Stage<__half>::BYTES>(grid, Q_THREADS, 1, st, p));
   if (sums) {
     host_count_launch();
     add_sums<<<(unsigned)((cols + 31) / 32), 512, 0, st>>>(p.sums, sums, cols, (int)tiles128(rows));
@@ -379,9 +380,8 @@ int amsim_mx_dequantize(void* stream, const void* data, long long rows, long lon
   const long long grid = p.gx * tiles128(rows);
   if (grid >= (1ll << 31)) return host_fail(AMSIM_ERR_UNSUPPORTED, "mx_dequantize: more than 2^31 tiles");
   cudaStream_t st = (cudaStream_t)stream;
-  const int smem = transposed ? Q_SMEM_T : Q_SMEM;
-  AMSIM_HOST_TRY(dtype == 0 ? launch(dequantise<float>, grid, Q_THREADS, smem, 1, st, p)
-                            : dtype == 1 ? launch(dequantise<__nv_bfloat16>, grid, Q_THREADS, smem, 1, st, p) : launch(dequantise<__half>, grid, Q_THREADS, smem, 1, st, p));
+  AMSIM_HOST_TRY(dtype == 0 ? launch<dequantise<float>, Q_SMEM_T>(grid, Q_THREADS, 1, st, p)
+                            : dtype == 1 ? launch<dequantise<__nv_bfloat16>, Q_SMEM_T>(grid, Q_THREADS, 1, st, p) : launch<dequantise<__half>, Q_SMEM_T>(grid, Q_THREADS, 1, st, p));
   return AMSIM_OK;
 }
 

@@ -705,10 +705,12 @@ static bool vector_ok(const NormParams& p, int v) {
          aligned(p.pre_b) && aligned(p.sum) && aligned(p.y) && aligned(p.dsum) && aligned(p.dy) && aligned(p.dx) && aligned(p.dblock) && aligned(p.dgate);
 }
 
-template <typename K>
-static cudaError_t launch(K kernel, const Plan& pl, int smem, cudaStream_t st, const NormParams& p) {
+constexpr int MOST_SMEM = 224 * 1024;  // dynamic; the static arrays have the rest of a CTA's 227 KB
+template <auto kernel>
+static cudaError_t launch(const Plan& pl, int smem, cudaStream_t st, const NormParams& p) {
   if (smem > 40 * 1024) {  // (48 KB with the static arrays)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = host_allow_smem(kernel, MOST_SMEM, done);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -737,16 +739,16 @@ static cudaError_t launch_t(NormParams& p, bool backward, int device, cudaStream
   if (backward) {
     constexpr int E = bwd_elems<T, LAYER, POST, GATE>();
     const int smem = smem_bytes<T, V, Places<LAYER, POST, GATE, true>::COUNT>(p, E, bwd->s.threads);
-    if (V > 1 && p.width == bwd->s.tpr * E * bwd->s.cluster) return launch(norm_bwd<T, V, LAYER, POST, GATE, (V > 1)>, *bwd, smem, st, p);
-    return launch(norm_bwd<T, V, LAYER, POST, GATE, false>, *bwd, smem, st, p);
+    if (V > 1 && p.width == bwd->s.tpr * E * bwd->s.cluster) return launch<norm_bwd<T, V, LAYER, POST, GATE, (V > 1)>>(*bwd, smem, st, p);
+    return launch<norm_bwd<T, V, LAYER, POST, GATE, false>>(*bwd, smem, st, p);
   }
   constexpr int E = fwd_elems<T, LAYER, POST, GATE>();
   Plan pl;
   if (!make_plan(p.rows, p.width, E, 512, 1, false, device, &pl)) return cudaErrorInvalidValue;
   p.tpr = pl.s.tpr; p.tpr_log = pl.s.tpr_log; p.cluster = pl.s.cluster; p.per_worker = pl.per_worker; p.workers = pl.workers;
   const int smem = smem_bytes<T, V, Places<LAYER, POST, GATE, false>::COUNT>(p, E, pl.s.threads);
-  if (V > 1 && p.width == pl.s.tpr * E * pl.s.cluster) return launch(norm_fwd<T, V, LAYER, POST, GATE, (V > 1)>, pl, smem, st, p);
-  return launch(norm_fwd<T, V, LAYER, POST, GATE, false>, pl, smem, st, p);
+  if (V > 1 && p.width == pl.s.tpr * E * pl.s.cluster) return launch<norm_fwd<T, V, LAYER, POST, GATE, (V > 1)>>(pl, smem, st, p);
+  return launch<norm_fwd<T, V, LAYER, POST, GATE, false>>(pl, smem, st, p);
 }
 
 template <typename T, int V, bool LAYER>

@@ -13,6 +13,7 @@ gradients.
 from __future__ import annotations
 
 import array
+import contextlib
 import ctypes as C
 import math
 
@@ -35,14 +36,17 @@ def _tensor(t, name: str, like: torch.Tensor = None) -> torch.Tensor:
     return t
 
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _call(device: torch.device, fn, *args) -> None:
     """``fn(current stream, ...)`` with `device` current; raises what the library reports."""
     idx = device.index
-    if idx == torch.cuda.current_device():
-        check(fn(torch._C._cuda_getCurrentRawStream(idx), *args))
+    if idx == _current_device():
+        check(fn(_current_stream(idx), *args))
     else:
         with torch.cuda.device(idx):
-            check(fn(torch._C._cuda_getCurrentRawStream(idx), *args))
+            check(fn(_current_stream(idx), *args))
 
 
 def _ptr(t):
@@ -180,7 +184,7 @@ def residual_norm_grad(dr, dy, x, stats, block=None, gate=None, gate_rows: int =
             if t is not None:
                 t.zero_()
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(device) if device.index != _current_device() else contextlib.nullcontext():
             size = lib.amsim_residual_norm_grad_workspace(rows, width, gate is not None, _TYPES[like.dtype], flags)
         ws = torch.empty(size, dtype=torch.uint8, device=device)
         _call(device, lib.amsim_residual_norm_grad, _ptr(dr), _ptr(dy), x.data_ptr(), _ptr(block), _ptr(gate), _ptr(post_w), _ptr(post_b),
