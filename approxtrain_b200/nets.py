@@ -10,7 +10,11 @@ around the custom ops).  Inputs are NHWC.
 * ``ResNet50AM``    profile/resnet50_lut.py:568-718 (bottleneck v1; the 3x3/2 max pool is unpadded, so
                     stage 2 runs at 55x55 for a 224x224 input); the final FC is an AM dense.
 * ``TransformerAM`` ammha/encoder.py, decoder.py, multihead_attention.py, positional_encoding.py:
-                    post-norm encoder/decoder, sinusoidal positions, token id 0 is padding.
+                    post-norm encoder/decoder, sinusoidal positions, token id 0 is padding.  Options beside the
+                    reference's form: ``fused_norms`` (each residual add and its LayerNorm in one launch, forward and
+                    backward), ``positions="rotary"`` (queries and keys of the self-attentions turned by their positions
+                    instead of sinusoids added to the embeddings), ``dense="mx"`` (dense layers in 4-bit floats,
+                    attention products through the table as before).
 """
 from __future__ import annotations
 
@@ -19,7 +23,7 @@ import math
 import torch
 from torch import nn
 
-from .layers import AMConv2D, BatchNormNHWC, ammatmul, denseam, nhwc_avg_pool, nhwc_max_pool
+from .layers import AMConv2D, BatchNormNHWC, ammatmul, denseam, densemx, nhwc_avg_pool, nhwc_max_pool, residual_norm, rotary
 
 
 class LeNet300100(nn.Module):
@@ -106,23 +110,43 @@ def _sinusoid(length, depth):
     return torch.cat([torch.sin(ang), torch.cos(ang)], dim=-1)
 
 
+def _dense(kind, lut, det):
+    """The dense layers of a Transformer: through the multiplier's table, or in 4-bit floats."""
+    if kind == "am":
+        return lambda i, o, **kw: denseam(i, o, mant_mul_lut=lut, deterministic=det, **kw)
+    if kind == "mx":
+        return densemx
+    raise ValueError(f"dense must be 'am' or 'mx', got {kind!r}")
+
+
+def _add_norm(norm, x, block, fused):
+    """``norm(x + block)``, in one launch or as the two ops."""
+    if fused:
+        return residual_norm(x, block, pre=(norm.weight, norm.bias), kind="layer", eps=norm.eps, need_sum=False)[1]
+    return norm(x + block)
+
+
 class _MHA(nn.Module):
-    def __init__(self, lut, h, d_k, d_v, d_model, det):
+    def __init__(self, lut, h, d_k, d_v, d_model, det, dense="am"):
         super().__init__()
-        kw = dict(mant_mul_lut=lut, deterministic=det)
+        new = _dense(dense, lut, det)
         self.h, self.d_k, self.lut, self.det = h, d_k, lut, det
         self.inv_scale = float(torch.tensor(1.0) / torch.tensor(math.sqrt(d_k), dtype=torch.float32))
-        self.wq = denseam(d_model, d_k, **kw)
-        self.wk = denseam(d_model, d_k, **kw)
-        self.wv = denseam(d_model, d_v, **kw)
-        self.wo = denseam(d_v, d_model, **kw)
+        self.wq = new(d_model, d_k)
+        self.wk = new(d_model, d_k)
+        self.wv = new(d_model, d_v)
+        self.wo = new(d_v, d_model)
 
     def _split(self, x):
         b, s, _ = x.shape
         return x.reshape(b, s, self.h, -1).permute(0, 2, 1, 3).contiguous()
 
-    def forward(self, q, k, v, mask=None):
-        q, k, v = self._split(self.wq(q)), self._split(self.wk(k)), self._split(self.wv(v))
+    def forward(self, q, k, v, mask=None, turn=None):
+        q, k, v = self.wq(q), self.wk(k), self._split(self.wv(v))
+        if turn is not None:   # (positions, frequencies)
+            q, k = (t.unflatten(-1, (self.h, -1)) for t in (q, k))
+            q, k = (t.flatten(-2) for t in rotary(q, turn[0], turn[1], k=k))
+        q, k = self._split(q), self._split(k)
         # scores are scaled by sqrt(d_k) with d_k as passed to the layer (multihead_attention.py:16-18)
         # (1 / sqrt(d_k) as one FP32 factor in the product's epilogue, K read transposed in place)
         scores = ammatmul(q, k, self.lut, self.det, transpose_b=True, alpha=self.inv_scale)
@@ -134,58 +158,75 @@ class _MHA(nn.Module):
 
 
 class _FFN(nn.Module):
-    def __init__(self, lut, d_ff, d_model, det):
+    def __init__(self, lut, d_ff, d_model, det, dense="am"):
         super().__init__()
-        self.f1 = denseam(d_model, d_ff, activation="relu", mant_mul_lut=lut, deterministic=det)
-        self.f2 = denseam(d_ff, d_model, mant_mul_lut=lut, deterministic=det)
+        new = _dense(dense, lut, det)
+        self.f1 = new(d_model, d_ff, activation="relu")
+        self.f2 = new(d_ff, d_model)
 
     def forward(self, x):
         return self.f2(self.f1(x))
 
 
 class _EncLayer(nn.Module):
-    def __init__(self, lut, h, d_k, d_v, d_model, d_ff, det):
+    def __init__(self, lut, h, d_k, d_v, d_model, d_ff, det, dense="am", fused=False):
         super().__init__()
-        self.mha = _MHA(lut, h, d_k, d_v, d_model, det)
+        self.mha = _MHA(lut, h, d_k, d_v, d_model, det, dense)
         self.n1 = nn.LayerNorm(d_model, eps=1e-3)
-        self.ffn = _FFN(lut, d_ff, d_model, det)
+        self.ffn = _FFN(lut, d_ff, d_model, det, dense)
         self.n2 = nn.LayerNorm(d_model, eps=1e-3)
+        self.fused = fused
 
-    def forward(self, x, pad_mask):
-        x = self.n1(x + self.mha(x, x, x, pad_mask))
-        return self.n2(x + self.ffn(x))
+    def forward(self, x, pad_mask, turn=None):
+        x = _add_norm(self.n1, x, self.mha(x, x, x, pad_mask, turn), self.fused)
+        return _add_norm(self.n2, x, self.ffn(x), self.fused)
 
 
 class _DecLayer(nn.Module):
-    def __init__(self, lut, h, d_k, d_v, d_model, d_ff, det):
+    def __init__(self, lut, h, d_k, d_v, d_model, d_ff, det, dense="am", fused=False):
         super().__init__()
-        self.mha1 = _MHA(lut, h, d_k, d_v, d_model, det)
+        self.mha1 = _MHA(lut, h, d_k, d_v, d_model, det, dense)
         self.n1 = nn.LayerNorm(d_model, eps=1e-3)
-        self.mha2 = _MHA(lut, h, d_k, d_v, d_model, det)
-        self.ffn = _FFN(lut, d_ff, d_model, det)
+        self.mha2 = _MHA(lut, h, d_k, d_v, d_model, det, dense)
+        self.ffn = _FFN(lut, d_ff, d_model, det, dense)
         self.n3 = nn.LayerNorm(d_model, eps=1e-3)
+        self.fused = fused
 
-    def forward(self, x, enc, look_mask, pad_mask):
-        a1 = self.n1(x + self.mha1(x, x, x, look_mask))
+    def forward(self, x, enc, look_mask, pad_mask, turn=None):
+        a1 = _add_norm(self.n1, x, self.mha1(x, x, x, look_mask, turn), self.fused)
         # the reference reuses add_norm1 for the second residual (ammha/decoder.py:41)
-        a2 = self.n1(a1 + self.mha2(a1, enc, enc, pad_mask))
-        return self.n3(a2 + self.ffn(a2))
+        a2 = _add_norm(self.n1, a1, self.mha2(a1, enc, enc, pad_mask), self.fused)
+        return _add_norm(self.n3, a2, self.ffn(a2), self.fused)
 
 
 class TransformerAM(nn.Module):
     def __init__(self, lut, vocab=8000, layers=6, d_model=512, heads=8, d_ff=2048, d_k=512, d_v=512,
-                 deterministic=False):
+                 deterministic=False, fused_norms=False, positions="sinusoidal", dense="am"):
         super().__init__()
-        self.d_model = d_model
+        if positions not in ("sinusoidal", "rotary"):
+            raise ValueError(f"positions must be 'sinusoidal' or 'rotary', got {positions!r}")
+        self.d_model, self.positions, self.head_dim = d_model, positions, d_k // heads
         self.src_emb = nn.Embedding(vocab, d_model, padding_idx=0)
         self.tgt_emb = nn.Embedding(vocab, d_model, padding_idx=0)
         self.register_buffer("pos", _sinusoid(2048, d_model), persistent=False)
-        self.enc = nn.ModuleList([_EncLayer(lut, heads, d_k, d_v, d_model, d_ff, deterministic) for _ in range(layers)])
-        self.dec = nn.ModuleList([_DecLayer(lut, heads, d_k, d_v, d_model, d_ff, deterministic) for _ in range(layers)])
-        self.out = denseam(d_model, vocab, mant_mul_lut=lut, deterministic=deterministic)
+        kw = dict(det=deterministic, dense=dense, fused=fused_norms)
+        self.enc = nn.ModuleList([_EncLayer(lut, heads, d_k, d_v, d_model, d_ff, **kw) for _ in range(layers)])
+        self.dec = nn.ModuleList([_DecLayer(lut, heads, d_k, d_v, d_model, d_ff, **kw) for _ in range(layers)])
+        self.out = _dense(dense, lut, deterministic)(d_model, vocab)
+        self._freqs = None
 
     def _embed(self, emb, ids):
-        return emb(ids) * math.sqrt(self.d_model) + self.pos[None, : ids.shape[1]]
+        x = emb(ids) * math.sqrt(self.d_model)
+        return x + self.pos[None, : ids.shape[1]] if self.positions == "sinusoidal" else x
+
+    def _turn(self, ids):
+        """What the self-attentions turn queries and keys by: (positions, frequencies), or None."""
+        if self.positions != "rotary":
+            return None
+        if self._freqs is None or self._freqs.inv_freq.device != ids.device:
+            from .ops import rotary_frequencies
+            self._freqs = rotary_frequencies(self.head_dim // 2 * 2, device=ids.device)
+        return torch.arange(ids.shape[1], device=ids.device), self._freqs
 
     def forward(self, src, tgt):
         pad_src = (src == 0).float()[:, None, None, :]
@@ -193,9 +234,11 @@ class TransformerAM(nn.Module):
         s = tgt.shape[1]
         look = torch.maximum(torch.triu(torch.ones(s, s, device=tgt.device), 1)[None, None], pad_tgt)
         x = self._embed(self.src_emb, src)
+        turn = self._turn(src)
         for layer in self.enc:
-            x = layer(x, pad_src)
+            x = layer(x, pad_src, turn)
         y = self._embed(self.tgt_emb, tgt)
+        turn = self._turn(tgt)
         for layer in self.dec:
-            y = layer(y, x, look, pad_src)
+            y = layer(y, x, look, pad_src, turn)
         return self.out(y)
