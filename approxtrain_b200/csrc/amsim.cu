@@ -11,6 +11,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <chrono>
+#include <condition_variable>
 #include <map>
 #include <mutex>
 #include <set>
@@ -525,6 +527,7 @@ struct CaptureRegion {
 };
 struct CaptureRegions {
   std::mutex mu;
+  std::condition_variable came_back;  // a spare region more
   std::vector<CaptureRegion*> used;   // by a capture or a graph; the newest of a stream last
   std::vector<CaptureRegion*> spare;
 };
@@ -538,6 +541,7 @@ void CUDART_CB region_released(void* p) {
   std::lock_guard<std::mutex> lk(r.mu);
   r.used.erase(std::find(r.used.begin(), r.used.end(), static_cast<CaptureRegion*>(p)));
   r.spare.push_back(static_cast<CaptureRegion*>(p));
+  r.came_back.notify_all();
 }
 
 // Calls that no capture allows in its strict modes: this thread's, for as long as the object lives, are allowed.
@@ -580,15 +584,24 @@ void* capture_region(cudaStream_t st, int device, size_t bytes) {
   CaptureRegions& r = capture_regions();
   CaptureRegion* region = nullptr;
   {
-    std::lock_guard<std::mutex> lk(r.mu);
-    for (size_t i = r.used.size(); i-- > 0;)
+    std::unique_lock<std::mutex> lk(r.mu);
+    bool others = false;  // regions of other captures
+    for (size_t i = r.used.size(); i-- > 0;) {
       if (r.used[i]->capture == id && r.used[i]->stream == st && r.used[i]->device == device && r.used[i]->bytes >= bytes)
         return r.used[i]->mem;
-    for (size_t i = 0; i < r.spare.size() && !region; ++i)
-      if (r.spare[i]->device == device && r.spare[i]->bytes >= bytes) {
-        region = r.spare[i];
-        r.spare.erase(r.spare.begin() + i);
-      }
+      others = others || (r.used[i]->capture != id && r.used[i]->device == device);
+    }
+    auto take = [&]() {
+      for (size_t i = 0; i < r.spare.size() && !region; ++i)
+        if (r.spare[i]->device == device && r.spare[i]->bytes >= bytes) {
+          region = r.spare[i];
+          r.spare.erase(r.spare.begin() + i);
+        }
+      return region != nullptr;
+    };
+    // A graph that is gone hands its region back on a thread of the driver, a moment later (once in some twenty captures
+    // right behind it the region was not there yet, and another 40 MB were taken).  A capture waits for that moment.
+    if (!take() && others) r.came_back.wait_for(lk, std::chrono::milliseconds(20), take);
   }
   if (!region) {
     // as large as any tensor-core launch takes, so that a stream rarely needs a second one
