@@ -14,9 +14,9 @@ DEFAULT_LIB_PATH = os.path.join(_PKG, "libamsim.so")
 # build libamsim_check.so (build_checked below); it is never rebuilt automatically.
 LIB_PATH = os.environ.get("AMSIM_LIBRARY") or DEFAULT_LIB_PATH
 CHECKED_LIB_PATH = os.path.join(_PKG, "libamsim_check.so")
-SOURCES = [os.path.join(_PKG, "csrc", f) for f in ("amsim.cu", "amsim_codes.cu", "amsim_norm.cu", "amsim_rotary.cu", "amsim_adamw.cu", "amsim_mx.cu")]
+SOURCES = [os.path.join(_PKG, "csrc", f) for f in ("amsim.cu", "amsim_codes.cu", "amsim_norm.cu", "amsim_norm_bf16.cu", "amsim_norm_f16.cu", "amsim_rotary.cu", "amsim_adamw.cu", "amsim_mx.cu")]
 HEADERS = [os.path.join(_PKG, "csrc", h) for h in ("amsim_kernels.cuh", "amsim_wide.cuh", "amsim_codes.cuh", "amsim_codes_launch.h",
-                                                   "amsim_factor.h", "amsim_host.h", "amsim_elem.cuh", "amsim_mx.cuh")] + [
+                                                   "amsim_factor.h", "amsim_host.h", "amsim_elem.cuh", "amsim_mx.cuh", "amsim_norm.cuh")] + [
            os.path.join(os.path.dirname(_PKG), "include", "amsim.h")]
 
 NVCC_FLAGS = [

@@ -32,6 +32,8 @@
 #ifndef AMSIM_SPLIT_TU
 #include "amsim_codes.cu"
 #include "amsim_norm.cu"
+#include "amsim_norm_bf16.cu"
+#include "amsim_norm_f16.cu"
 #include "amsim_rotary.cu"
 #include "amsim_adamw.cu"
 #include "amsim_mx.cu"

@@ -1,4 +1,5 @@
-// Loads and stores of V consecutive elements (16 bytes, or one element) as FP32, for kernels over float, bfloat16 and half.
+// Loads and stores of V consecutive elements as FP32, for kernels over float, bfloat16 and half: V elements at a multiple of
+// their size together (up to 16 bytes at a time; two floats one by one).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -25,6 +26,9 @@ __device__ __forceinline__ void load_vec(const void* base, long long at, float (
   const T* p = static_cast<const T*>(base) + at;
   if constexpr (V == 1) {
     o[0] = elem_to_float(*p);
+  } else if constexpr (sizeof(T) == 4 && V < 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = p[i];
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
@@ -32,14 +36,16 @@ __device__ __forceinline__ void load_vec(const void* base, long long at, float (
       o[4 * i] = v.x; o[4 * i + 1] = v.y; o[4 * i + 2] = v.z; o[4 * i + 3] = v.w;
     }
   } else {
-    static_assert(V % 2 == 0, "pairs");
+    static_assert(V == 2 || V == 4 || V == 8, "4, 8 or 16 bytes");
     uint32_t w[V / 2];
     if constexpr (V == 8) {
       const uint4 v = *reinterpret_cast<const uint4*>(p);
       w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else {
+    } else if constexpr (V == 4) {
       const uint2 v = *reinterpret_cast<const uint2*>(p);
       w[0] = v.x; w[1] = v.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
@@ -66,6 +72,9 @@ __device__ __forceinline__ void store_vec(void* base, long long at, const float 
   T* p = static_cast<T*>(base) + at;
   if constexpr (V == 1) {
     *p = elem_from_float<T>(o[0]);
+  } else if constexpr (sizeof(T) == 4 && V < 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = o[i];
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) *reinterpret_cast<float4*>(p + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -77,7 +86,8 @@ __device__ __forceinline__ void store_vec(void* base, long long at, const float 
       memcpy(&w[i], pair, 4);
     }
     if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
 }
 

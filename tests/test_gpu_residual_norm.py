@@ -201,6 +201,19 @@ def test_unaligned_and_strided_tensors():
             _check(a, rnd, t)
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_of_four_byte_chunks_and_of_single_elements(t):
+    """Even lengths that are no multiple of 16 bytes, odd ones, and tensors at half of a chunk's alignment."""
+    for width in (6, 130, 3950, 1001):
+        for gate, post in (("full", True), ("sequence", False), (None, True)):
+            a, rnd = _make((5, 9, width), t, "layer", post, gate, True, 0.5, True, torch.float32, seed=width)
+            _check(a, rnd, t)
+    off = lambda v: torch.empty(v.numel() + 1, dtype=v.dtype, device="cuda")[1:].view(v.shape).copy_(v.detach())
+    a, rnd = _make((6, 5, 66), t, "rms", True, "width", True, 1.0, True, torch.float32)
+    a.update(x=off(a["x"]), pre=tuple(None if v is None else off(v) for v in a["pre"]))
+    _check(a, rnd, t)
+
+
 def test_the_formula_agrees_with_differences():
     """The 64-bit gradient above against central differences of the 64-bit forward pass."""
     g = torch.Generator().manual_seed(0)
