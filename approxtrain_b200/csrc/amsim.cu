@@ -260,6 +260,7 @@ int host_stuck_word(int device, unsigned** word) {
   return AMSIM_OK;
 }
 int host_report_stuck(int device) { return report_stuck(device); }
+bool host_no_tries() { return sw().codes_spin == 0; }
 
 }  // namespace amsim
 

@@ -17,6 +17,7 @@ int host_device();
 // AMSIM_ERR_CUDA by the next call that asks.
 int host_stuck_word(int device, unsigned** word);
 int host_report_stuck(int device);
+bool host_no_tries();  // AMSIM_CODES_SPIN=0: bounded waits give up at once (for the test of the report)
 
 // Lets `kernel` take up to `bytes` of dynamic shared memory: asked for once per device and kernel (`done`: a word of the
 // kernel's own, one bit a device).

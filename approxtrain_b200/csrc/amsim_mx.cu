@@ -405,6 +405,7 @@ int amsim_mx_matmul(void* stream, const void* a, const void* b, long long m, lon
   p.last_steps = k == 0 ? 1 : (int)((k - (long long)(p.kt - 1) * 256 + 63) / 64);
   p.chunk = dtype == 0 ? 8 : 32;
   p.relu = act == AMSIM_ACT_RELU;
+  p.no_tries = host_no_tries();
   if ((long long)((p.a_tiles + 1) / 2 + 1) * p.b_tiles >= (1ll << 30)) return host_fail(AMSIM_ERR_UNSUPPORTED, "mx_matmul: more than 2^30 tiles");
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;

@@ -26,7 +26,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
-from .train_ops import _NormArgs, _norm_forward
+from .train_ops import _NormArgs, _norm_backward, _norm_forward
 
 
 class GradSink:
@@ -408,8 +408,8 @@ class _ResidualNormFn(torch.autograd.Function):
         x, stats, block, gate, post_w, post_b, pre_w, pre_b = ctx.saved_tensors
         gate_rows, scale, flags = ctx.cfg
         dr, dy = (None if g is None else g.contiguous() for g in (dr, dy))
-        grads = ops.residual_norm_grad(dr, dy, x, stats, block, gate, gate_rows, scale, post_w, post_b, pre_w, pre_b, flags,
-                                       wants=ctx.needs_input_grad[:7])
+        grads = _norm_backward(dr, dy, x, stats, block, gate, gate_rows, scale, post_w, post_b, pre_w, pre_b, flags,
+                               wants=ctx.needs_input_grad[:7])
         return (*(g if want else None for g, want in zip(grads, ctx.needs_input_grad)), None, None)
 
 
@@ -512,10 +512,12 @@ class _MXDenseFn(torch.autograd.Function):
 
 def mxdense(x, w, bias=None, activation=None):
     """``act(x w + bias)`` on the last axis with the products in 4-bit floats (``ops.mx_matmul``), forward and backward; x [..., in],
-    w [in, out], float32, bfloat16 or float16; bias float32.  ``activation``: None or "relu"."""
+    w [in, out], bias [out], float32, bfloat16 or float16.  ``activation``: None or "relu"."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[0]:
         raise ValueError(f"x [..., in] and w [in, out] expected, got {list(x.shape)} and {list(w.shape)}")
     lead = x.shape[:-1]
+    if bias is not None and bias.dtype != torch.float32:
+        bias = bias.float()
     y = _MXDenseFn.apply(x.reshape(-1, x.shape[-1]), w, bias, activation)
     return y.reshape(*lead, w.shape[1])
 
@@ -544,7 +546,8 @@ class densemx(nn.Module):
     def forward(self, x):
         fused = self.activation if self.activation in (None, "linear", "relu") else None
         if self._frozen is not None:
-            y = ops.mx_matmul(ops.mx_quantize(x.reshape(-1, x.shape[-1])), self._frozen, bias=self.bias, activation=fused, out_dtype=x.dtype)
+            y = ops.mx_matmul(ops.mx_quantize(x.reshape(-1, x.shape[-1])), self._frozen, bias=self.bias.float() if self.bias is not None else None, activation=fused,
+                              out_dtype=x.dtype)
             y = y.reshape(*x.shape[:-1], self.kernel.shape[1])
         else:
             y = mxdense(x, self.kernel, self.bias, fused)

@@ -23,6 +23,10 @@ class MXTensor:
 
     def __init__(self, data: torch.Tensor, shape, axis: int):
         self.data, self.shape, self.axis = data, tuple(shape), axis
+        if len(self.shape) != 2 or axis not in (0, 1):
+            raise ValueError(f"a matrix and one of its axes (0, 1) expected, got {self.shape}, {axis}")
+        if not data.is_cuda or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != lib.amsim_mx_bytes(self.rows, self.k):
+            raise ValueError(f"data must be {lib.amsim_mx_bytes(self.rows, self.k)} contiguous bytes on a CUDA device")
 
     @property
     def rows(self) -> int:

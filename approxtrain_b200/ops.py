@@ -32,12 +32,12 @@ import torch
 from . import _lib
 from ._lib import AmsimError, lib, check
 from .mx import MXTensor, mx_matmul, mx_quantize, mx_quantize_both
-from .train_ops import AdamWState, RotaryFrequencies, adamw_step, residual_norm, residual_norm_grad, rotary, rotary_frequencies
+from .train_ops import AdamWState, RotaryFrequencies, adamw_step, residual_norm, rotary, rotary_frequencies
 
 __all__ = [
     "AMLut", "get_lut", "am_multiply", "conv2d_geometry", "convam", "convam_input_grad", "convam_filter_grad",
     "denseam", "denseam_grad", "matmulam", "convam_bias_act", "denseam_bias_act", "bias_grad", "AmsimError",
-    "residual_norm", "residual_norm_grad", "rotary", "rotary_frequencies", "RotaryFrequencies", "adamw_step", "AdamWState",
+    "residual_norm", "rotary", "rotary_frequencies", "RotaryFrequencies", "adamw_step", "AdamWState",
     "mx_quantize", "mx_quantize_both", "mx_matmul", "MXTensor",
 ]
 
@@ -457,7 +457,7 @@ def _install_nvtx_ranges() -> None:
         return
     g = globals()
     for name in ("am_multiply", "convam", "convam_bias_act", "denseam_bias_act", "convam_input_grad",
-                 "convam_filter_grad", "denseam", "denseam_grad", "matmulam", "bias_grad", "residual_norm", "residual_norm_grad", "rotary", "adamw_step",
+                 "convam_filter_grad", "denseam", "denseam_grad", "matmulam", "bias_grad", "residual_norm", "rotary", "adamw_step",
                  "mx_quantize", "mx_quantize_both", "mx_matmul"):
         fn = g[name]
 

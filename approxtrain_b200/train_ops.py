@@ -161,9 +161,9 @@ def residual_norm(x, block=None, gate=None, scale: float = 1.0, post=None, pre=N
     return r, y
 
 
-def residual_norm_grad(dr, dy, x, stats, block=None, gate=None, gate_rows: int = 0, scale: float = 1.0, post_w=None, post_b=None,
+def _norm_backward(dr, dy, x, stats, block=None, gate=None, gate_rows: int = 0, scale: float = 1.0, post_w=None, post_b=None,
                        pre_w=None, pre_b=None, flags: int = NORM_PRE, wants=(True,) * 7):
-    """Gradients (x, block, gate, post weight, post bias, pre weight, pre bias) of ``residual_norm`` from those of its
+    """Gradients (x, block, gate, post weight, post bias, pre weight, pre bias) of a checked forward pass from those of its
     outputs (either may be None); ``stats`` is the forward pass's, ``wants`` says which are computed.  The sum is made
     again from x and block, unrounded.  Where x and block are only added (no norm after the block, no gate, scale 1) the block's gradient is x's tensor."""
     like = x
@@ -278,6 +278,8 @@ def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half",
                 raise ValueError(f"{name} must have a dense last axis to be rotated in place")
             if t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
                 raise ValueError(f"{name} must not be an expanded tensor to be rotated in place")
+            if t is not None and t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{name} requires a gradient: it cannot be rotated in place (layers.rotary keeps gradients)")
         _rotary_heads(q, "q")
     if not isinstance(freqs, RotaryFrequencies):
         raise TypeError("freqs must be RotaryFrequencies (rotary_frequencies)")
@@ -301,6 +303,8 @@ def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half",
     flags = (ROTARY_INTERLEAVED if layout == "interleaved" else 0) | (ROTARY_INVERSE if inverse else 0) | (ROTARY_POS32 if positions.dtype == torch.int32 else 0)
     _call(q.device, lib.amsim_rotary, q.data_ptr(), out.data_ptr(), q.shape[-2], _ptr(k_), _ptr(out2), k_.shape[-2] if k_ is not None else 0,
           positions.data_ptr(), freqs.inv_freq.data_ptr(), batch, seq, q.shape[-1], freqs.rotary_dim, strides, freqs.scale, _TYPES[q.dtype], flags)
+    if inplace:  # (a graph that has saved q or k notices)
+        torch.autograd.graph.increment_version([q] if k is None else [q, k])
     return out if k is None else (out, out2)
 
 
@@ -429,9 +433,12 @@ def adamw_step(params, grads, state: AdamWState, lr, betas=(0.9, 0.999), eps: fl
     lr, lr_at = _rate(lr, "lr", state.device)
     scale, scale_at = _rate(grad_scale, "grad_scale", state.device)
     p_at, g_at = array.array("Q", map(_data_ptr, params)), array.array("Q", map(_data_ptr, grads))
+    if len(set(p_at)) < n and len({a for a, k in zip(p_at, state.sizes) if k}) < sum(map(bool, state.sizes)):
+        raise ValueError("a parameter is listed twice (tied weights are updated once)")
     if state.bits == 32:
         m, ms, v, vs = state.exp_avg.data_ptr(), None, state.exp_avg_sq.data_ptr(), None
     else:
         m, ms, v, vs = (getattr(state, k).data_ptr() for k in state._moments)
     _call(state.device, lib.amsim_adamw, n, _address(p_at), _address(g_at), _address(state._sizes), _address(decay), m, ms, v, vs,
           state._counter.data_ptr(), lr, lr_at, b1, b2, eps, scale, scale_at, seed & 0xFFFFFFFF, _TYPES[state.dtype], _TYPES[types.pop()], state.bits)
+    torch.autograd.graph.increment_version(params)  # (a graph that has saved a parameter notices)

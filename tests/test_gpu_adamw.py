@@ -230,6 +230,21 @@ def test_refusals():
         with pytest.raises((ValueError, TypeError)):
             f()
     assert int(st.step) == 0
+    tied = torch.zeros(8, device="cuda")
+    two = ops.AdamWState([tied, tied])
+    with pytest.raises(ValueError, match="twice"):
+        ops.adamw_step([tied, tied], [g[0], g[0]], two, 0.1)
+    none = [torch.zeros(0, device="cuda"), torch.zeros(0, device="cuda"), tied]
+    ops.adamw_step(none, [torch.zeros_like(t) for t in none], ops.AdamWState(none), 0.1)     # empty tensors share an address
+
+
+def test_a_graph_that_saved_a_parameter_notices_the_step():
+    from approxtrain_b200 import ops
+    p = torch.ones(8, device="cuda", requires_grad=True)
+    y = (p * p).sum()
+    ops.adamw_step([p], [torch.ones(8, device="cuda")], ops.AdamWState([p]), 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 def test_trainer():

@@ -257,8 +257,44 @@ def test_captured():
     assert all(torch.equal(u, v) for u, v in zip(got, step()))
 
 
+def test_a_wait_that_runs_out_is_reported_by_the_next_call(monkeypatch):
+    """With no tries at all every warp gives up at its first wait: the launch ends, and the next call says so, once."""
+    from approxtrain_b200 import _lib, ops
+    shapes = [(10, 300, 300), (16, 128, 8192), (200, 500, 300), (2048, 2048, 512)]     # one CTA a tile, shared by several, pairs
+    cases = [(ops.mx_quantize(_rand(m, k)), ops.mx_quantize(_rand(n, k, seed=1))) for m, n, k in shapes]
+    want = [ops.mx_matmul(a, b) for a, b in cases]
+    for (a, b), w in zip(cases, want):
+        monkeypatch.setenv("AMSIM_CODES_SPIN", "0")
+        _lib.lib.amsim_debug_reload_env()
+        try:
+            ops.mx_matmul(a, b)
+            torch.cuda.synchronize()
+        finally:
+            monkeypatch.delenv("AMSIM_CODES_SPIN")
+            _lib.lib.amsim_debug_reload_env()
+        with pytest.raises(ops.AmsimError, match="gave up waiting"):
+            ops.mx_matmul(a, b)
+        assert torch.equal(ops.mx_matmul(a, b), w)
+    assert _lib.lib.amsim_async_status() == 0
+
+
+def test_a_layer_in_bf16():
+    from approxtrain_b200 import layers
+    m = layers.densemx(64, 32, activation="relu").cuda().bfloat16()
+    x = _rand(5, 64, t=torch.bfloat16)
+    y = m(x)
+    y.sum().backward()
+    assert y.dtype == torch.bfloat16 and m.bias.grad.dtype == torch.bfloat16 and m.kernel.grad.dtype == torch.bfloat16
+    with torch.no_grad():
+        assert torch.equal(m.freeze()(x), y)
+
+
 def test_refusals():
     from approxtrain_b200 import layers, ops
+    with pytest.raises(ValueError):
+        ops.MXTensor(torch.zeros(100, dtype=torch.uint8, device="cuda"), (4, 64), 1)
+    with pytest.raises(ValueError):
+        ops.MXTensor(torch.zeros(17408, dtype=torch.uint8, device="cuda"), (4, 64), 2)
     x = torch.zeros(4, 64, device="cuda")
     q = ops.mx_quantize(x)
     for bad in (lambda: ops.mx_quantize(x.double()), lambda: ops.mx_quantize(x[0]), lambda: ops.mx_quantize(x, axis=2), lambda: ops.mx_matmul(q, x),

@@ -117,6 +117,11 @@ def test_strided_tensors_and_in_place():
             assert torch.equal(joint, was)                                           # nothing beside it was written
         with pytest.raises(ValueError):
             ops.rotary(last, positions, freqs, inplace=True)
+        with pytest.raises(ValueError, match="gradient"):
+            ops.rotary(packed.clone().requires_grad_(), positions, freqs, inplace=True)
+        version = packed._version
+        ops.rotary(packed, positions, freqs, inplace=True)
+        assert packed._version == version + 1
         with pytest.raises(ValueError):
             ops.rotary(packed[:1].expand(9, 4, 48), positions, freqs, inplace=True)
 
