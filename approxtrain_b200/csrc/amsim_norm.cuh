@@ -294,6 +294,8 @@ struct Walk {
   }
 };
 
+// Forward.  8192 x 512 FP32, x + block and a layer norm: 11.7 us (4.3 TB/s; 50 MB from and to memory).  16384 x 2048 bf16 with both
+// rms norms, a gate per sequence and the sum written: 59 us (4.6 TB/s), issuing instructions half of the time.
 template <typename T, int V, bool LAYER, bool POST, int GATE, int E, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_fwd(const __grid_constant__ NormParams p) {
   constexpr int N = E / V;
@@ -433,6 +435,8 @@ __device__ __forceinline__ void flush_block(float (&acc)[N][V], const Cols<V, FU
   }
 }
 
+// Backward.  The same cases: 14.7 us (4.6 TB/s) and 5.1 us of norm_reduce; 120 us (3.3 TB/s) and 6 us.  The second is bound by the issue of
+// instructions, about 70 an element: conversions, 28 of arithmetic, and a row's fixed share (two row sums, addresses) over 8 elements.
 template <typename T, int V, bool LAYER, bool POST, int GATE, int E, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ NormParams p) {
   constexpr int N = E / V;
