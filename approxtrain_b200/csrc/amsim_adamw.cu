@@ -156,14 +156,12 @@ __device__ __forceinline__ void half_chunk32(const Entry& e, const Common& c, lo
   }
 }
 
-// The code of |a| / scale in the top byte (below it garbage), rounded up where the bits below the code's and 16 random ones
-// carry: E4M3's codes are the FP32 pattern's top bits less an offset.  Below 2^-6 codes are 2^-9 apart, as they are from 2^-6 to
-// 2^-5: the same bits after adding 2^-6, with 8 codes more to take off.  A value that the clamp holds at 448 has no bits to carry.
-// random16: the random bits times 16, plus 8.
+// The code of |a| / scale in the top byte (below it garbage), rounded up where the bits below the code's and 16 random ones carry.
+// Times 2^-120 an E4M3 value's FP32 pattern begins with its code, values below 2^-6 (E4M3's subnormal ones) among FP32's: no cases.
+// A value that the clamp holds at 448 has no bits to carry.  random16: the random bits times 16, plus 8.
 __device__ __forceinline__ uint32_t round8(float a, float inv, uint32_t random16, bool at_least) {
-  const float q = fminf(fabsf(a) * inv, 448.f);
-  const bool low = q < 0x1p-6f;
-  uint32_t code = __float_as_uint(low ? q + 0x1p-6f : q) + random16 - (low ? 968u << 20 : 960u << 20);
+  const float q = fminf(fabsf(a) * inv, 448.f) * 0x1p-120f;
+  uint32_t code = __float_as_uint(q) + random16;
   if (at_least) code = max(code, q > 0.f ? 1u << 20 : 0u);
   return code << 4;
 }

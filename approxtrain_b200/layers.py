@@ -26,6 +26,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import ops
+from .mx import _tiles
 from .train_ops import _NormArgs, _norm_backward, _norm_forward
 
 
@@ -505,8 +506,8 @@ class _MXDenseFn(torch.autograd.Function):
             if want_b:
                 torch.sum(g, 0, dtype=torch.float32, out=db)
             g_rows, g_cols = (ops.mx_quantize(g) if want_x else None), (ops.mx_quantize(g, axis=0) if want_w else None)
-        dx = ops.mx_matmul(g_rows, ops.MXTensor(w_data, w_shape, 1), out_dtype=x_type) if want_x else None
-        dw = ops.mx_matmul(ops.MXTensor(x_data, x_shape, 0), g_cols, out_dtype=w_type) if want_w else None
+        dx = ops.mx_matmul(g_rows, _tiles(w_data, w_shape, 1), out_dtype=x_type) if want_x else None
+        dw = ops.mx_matmul(_tiles(x_data, x_shape, 0), g_cols, out_dtype=w_type) if want_w else None
         return dx, dw, db, None
 
 

@@ -17,6 +17,21 @@ from ._lib import ACT_NONE, ACT_RELU, lib
 from .train_ops import _TYPES, _call, _tensor
 
 
+_TILE = 17408   # bytes of a tile: 128 rows x 256 elements
+
+
+def _bytes(rows: int, k: int) -> int:
+    """``amsim_mx_bytes``."""
+    return -(-rows // 128) * (-(-k // 256) or 1) * _TILE
+
+
+def _tiles(data: torch.Tensor, shape, axis: int) -> "MXTensor":
+    """An MXTensor of tiles that the library has written."""
+    t = object.__new__(MXTensor)
+    t.data, t.shape, t.axis = data, tuple(shape), axis
+    return t
+
+
 class MXTensor:
     """A matrix in 4-bit floats.  ``shape``: of the matrix as it was; ``axis``: the quantised one (1: blocks of 32 along the
     rows' elements, 0: along the columns').  ``data``: the library's tiles (uint8)."""
@@ -25,8 +40,8 @@ class MXTensor:
         self.data, self.shape, self.axis = data, tuple(shape), axis
         if len(self.shape) != 2 or axis not in (0, 1):
             raise ValueError(f"a matrix and one of its axes (0, 1) expected, got {self.shape}, {axis}")
-        if not data.is_cuda or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != lib.amsim_mx_bytes(self.rows, self.k):
-            raise ValueError(f"data must be {lib.amsim_mx_bytes(self.rows, self.k)} contiguous bytes on a CUDA device")
+        if not data.is_cuda or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != _bytes(self.rows, self.k):
+            raise ValueError(f"data must be {_bytes(self.rows, self.k)} contiguous bytes on a CUDA device")
 
     @property
     def rows(self) -> int:
@@ -61,14 +76,14 @@ def _matrix(x):
 
 def _quantize(x, along: bool, across: bool, sums=None):
     rows, cols = x.shape
-    one = torch.empty(lib.amsim_mx_bytes(rows, cols), dtype=torch.uint8, device=x.device) if along else None
-    two = torch.empty(lib.amsim_mx_bytes(cols, rows), dtype=torch.uint8, device=x.device) if across else None
-    size = lib.amsim_mx_quantize_workspace(rows, cols) if sums is not None else 0
+    one = torch.empty(_bytes(rows, cols), dtype=torch.uint8, device=x.device) if along else None
+    two = torch.empty(_bytes(cols, rows), dtype=torch.uint8, device=x.device) if across else None
+    size = -(-rows // 128) * cols * 4 if sums is not None else 0   # (amsim_mx_quantize_workspace)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     if (along and rows) or (across and cols):
         _call(x.device, lib.amsim_mx_quantize, x.data_ptr(), rows, cols, _TYPES[x.dtype], one.data_ptr() if along else None,
               two.data_ptr() if across else None, sums.data_ptr() if sums is not None else None, ws.data_ptr() if size else None, size)
-    return (MXTensor(one, (rows, cols), 1) if along else None), (MXTensor(two, (rows, cols), 0) if across else None)
+    return (_tiles(one, (rows, cols), 1) if along else None), (_tiles(two, (rows, cols), 0) if across else None)
 
 
 def mx_quantize(x: torch.Tensor, axis: int = -1) -> MXTensor:

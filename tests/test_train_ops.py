@@ -153,6 +153,11 @@ def test_mx_refusals(L):
     with pytest.raises(ValueError, match="CUDA"):
         ops.mx_quantize(torch.zeros(2, 4))
     p = 1 << 20
+    from approxtrain_b200 import mx
+    for rows in (0, 1, 127, 128, 129, 5000):
+        for k in (0, 1, 255, 256, 257, 9000):
+            assert mx._bytes(rows, k) == L.lib.amsim_mx_bytes(rows, k)
+            assert -(-rows // 128) * k * 4 == L.lib.amsim_mx_quantize_workspace(rows, k)
     d, m = L.lib.amsim_mx_dequantize, L.lib.amsim_mx_matmul
 
     def q(stream, x, rows, cols, dtype, along, across, sums=None, ws=None, size=0):
