@@ -139,7 +139,7 @@ struct Cols {
   __device__ __forceinline__ bool ok(int c) const { return FULL || at(c) < width; }
 };
 
-// Rows fetched ahead of their use, each thread its own chunks of 16 or 4 bytes: stage, tensor, chunk.  Single 16-bit elements (rows of
+// Rows fetched ahead of their use, each thread its own chunks of 16, 8 or 4 bytes: stage, tensor, chunk.  Single 16-bit elements (rows of
 // odd length) are loaded when they are needed.
 template <typename T, int V, int N, bool FULL>
 struct Ahead {
@@ -163,6 +163,7 @@ struct Ahead {
     for (int c = 0; c < N; ++c) {
       if (cols.ok(c)) {
         if constexpr (CHUNK == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        else if constexpr (CHUNK == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
         else if constexpr (CHUNK == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
       }
       from += cols.step;
@@ -183,6 +184,9 @@ struct Ahead {
       uint32_t w[4];
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place(stage, k, c)) : "memory");
       unpack16<T, V>(w, o);
+    } else if constexpr (CHUNK == 8) {
+      static_assert(sizeof(T) == 4, "two floats");
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(o[0]), "=f"(o[1]) : "r"(place(stage, k, c)) : "memory");
     } else if constexpr (CHUNK == 4) {
       uint32_t w;
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(place(stage, k, c)) : "memory");
@@ -837,13 +841,13 @@ static cudaError_t launch_v(NormParams& p, bool backward, bool layer, bool post,
   return layer ? launch_l<T, V, true>(p, backward, post, gate, device, st, bwd) : launch_l<T, V, false>(p, backward, post, gate, device, st, bwd);
 }
 
-// Chunks of 16 bytes where width and addresses allow them, else of 4, else single elements.  (Rows of 3950 FP32, N_post and a gate of
-// every row, forward and backward: 1241 us with single elements loaded when needed, 618 us with chunks of 4 bytes fetched ahead.)
+// Chunks of 16 bytes where width and addresses allow them, else two elements, else single ones.  (Rows of 3950 FP32, N_post and a gate of
+// every row, forward and backward: 1241 us with single elements loaded when needed, 618 us with them fetched ahead, 435 us in twos.)
 template <typename T>
 cudaError_t launch_type(NormParams& p, bool backward, bool layer, bool post, int gate, int device, cudaStream_t st, const Plan* bwd) {
-  constexpr int V = 16 / sizeof(T), SMALL = 4 / sizeof(T);
+  constexpr int V = 16 / sizeof(T);
   if (chunks_ok(p, V, 16)) return launch_v<T, V>(p, backward, layer, post, gate, device, st, bwd);
-  if (SMALL > 1 && chunks_ok(p, SMALL, 4)) return launch_v<T, SMALL>(p, backward, layer, post, gate, device, st, bwd);
+  if (chunks_ok(p, 2, 2 * sizeof(T))) return launch_v<T, 2>(p, backward, layer, post, gate, device, st, bwd);
   return launch_v<T, 1>(p, backward, layer, post, gate, device, st, bwd);
 }
 
