@@ -46,6 +46,11 @@ struct NormParams {
   int pre;
 };
 
+// The CTAs of a cluster meet before one writes another's shared memory: only then is it known that all of them have begun.  The arrival
+// comes before the first loads and the wait behind them, so that nobody waits for long.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // What a gate is to the kernels: none; rows shared by several rows, kept like the weights; or one row for each row, fetched ahead.
 constexpr int GATE_NONE = 0, GATE_SHARED = 1, GATE_ROWS = 2;
 
@@ -76,7 +81,8 @@ struct RowSum {
       asm volatile("{.reg .b32 r; mapa.shared::cluster.u32 r, %0, %1; st.shared::cluster.f32 [r], %2; st.shared::cluster.f32 [r + 32], %3;}" ::"r"(at),
                    "r"(threadIdx.x), "f"(a), "f"(b) : "memory");
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
   }
   __device__ __forceinline__ static void add_lanes(float& a, float& b, bool both, int lanes) {
     for (int o = lanes >> 1; o; o >>= 1) {
@@ -312,6 +318,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_fwd(const __grid_constant__ 
   RowSum sum{red[p.tpr > 32 ? group : 0], peers, p.tpr, p.cluster, rank, group, group * p.tpr >> 5, 0};
   const Cols<V, FULL> cols{(rank * N * p.tpr + t) * V, p.tpr * V, p.width};
   Walk w(p, (long long)(blockIdx.x / p.cluster) * groups + group);
+  if (p.cluster > 1) cluster_arrive();
   A in(p, smem);
   const Kept<V, N, FULL> kept(smem + A::bytes(p.n_in, blockDim.x));
   long long to_fetch = w.last - w.row, fetch_at = w.at + cols.first;
@@ -335,6 +342,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_fwd(const __grid_constant__ 
     kept.keep(P::POST_W, p.post_w, 0, w32, type16<T>(), 1.f, cols);
     if (LAYER) kept.keep(P::POST_B, p.post_b, 0, w32, type16<T>(), 0.f, cols);
   }
+  if (p.cluster > 1) cluster_wait();
   bool new_gate = true;
   for (long long i = 0; i < p.per_worker; ++i, in.next()) {  // (the same trips for all threads)
     const bool live = w.live();
@@ -460,6 +468,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
   for (int c = 0; c < N; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = dpw[c][e] = dpb[c][e] = dg[c][e] = 0.f;
+  if (p.cluster > 1) cluster_arrive();
   A in(p, smem);
   const Kept<V, N, FULL> kept(smem + A::bytes(p.n_in, blockDim.x));
   long long to_fetch = w.last - w.row, fetch_at = w.at + cols.first;
@@ -488,6 +497,7 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ 
     if (GATE == GATE_SHARED) kept.read(P::GATE_V, c, gv);
     else in.read(p.in_gate, c, p.gate, w.at, cols, gv);
   };
+  if (p.cluster > 1) cluster_wait();
   bool new_gate = true;
   for (long long i = 0; i < p.per_worker; ++i, in.next()) {  // (the same trips for all threads)
     const bool live = w.live();
