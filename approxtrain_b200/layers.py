@@ -525,7 +525,7 @@ def mxdense(x, w, bias=None, activation=None):
 
 class densemx(nn.Module):
     """Dense layer in 4-bit floats: the counterpart of ``denseam`` with the hardware's block-scaled products instead of a
-    multiplier's table.  ``freeze()`` keeps the weights quantised for inference."""
+    multiplier's table.  ``freeze()`` keeps the weights quantised for inference (under ``torch.no_grad()``)."""
 
     def __init__(self, in_features, units, activation=None, use_bias=True, kernel_initializer="glorot_uniform"):
         super().__init__()
@@ -535,8 +535,10 @@ class densemx(nn.Module):
         self._frozen = None
 
     def freeze(self):
-        """Quantises the weights once; later calls use them until ``train()`` is called."""
-        self._frozen = ops.mx_quantize(self.kernel.detach(), axis=0)
+        """Quantises the weights once.  Calls that record no gradient use them until ``train()`` is called, a state is loaded, the
+        module is moved or ``kernel`` is another parameter; a change of its elements in place does not reach them.  Calls that do
+        record one compute with ``kernel``, as without ``freeze()``."""
+        self._frozen = ops.mx_quantize(self.kernel.detach(), axis=0), self.kernel
         return self.eval()
 
     def train(self, mode=True):
@@ -544,11 +546,20 @@ class densemx(nn.Module):
             self._frozen = None
         return super().train(mode)
 
+    def _load_from_state_dict(self, *args, **kw):
+        self._frozen = None
+        super()._load_from_state_dict(*args, **kw)
+
+    def _apply(self, *args, **kw):
+        self._frozen = None
+        return super()._apply(*args, **kw)
+
     def forward(self, x):
         fused = self.activation if self.activation in (None, "linear", "relu") else None
-        if self._frozen is not None:
-            y = ops.mx_matmul(ops.mx_quantize(x.reshape(-1, x.shape[-1])), self._frozen, bias=self.bias.float() if self.bias is not None else None, activation=fused,
-                              out_dtype=x.dtype)
+        recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.kernel, self.bias))
+        if self._frozen is not None and self._frozen[1] is self.kernel and not recorded:
+            y = ops.mx_matmul(ops.mx_quantize(x.reshape(-1, x.shape[-1])), self._frozen[0], bias=self.bias.float() if self.bias is not None else None,
+                              activation=fused, out_dtype=x.dtype)
             y = y.reshape(*x.shape[:-1], self.kernel.shape[1])
         else:
             y = mxdense(x, self.kernel, self.bias, fused)

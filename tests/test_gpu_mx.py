@@ -303,3 +303,48 @@ def test_refusals():
                 lambda: q.dequantize(torch.int32), lambda: layers.mxdense(x, torch.zeros(32, 4, device="cuda"))):
         with pytest.raises((ValueError, TypeError)):
             bad()
+
+
+def test_frozen_weights_follow_loaded_moved_and_replaced_ones():
+    from approxtrain_b200 import layers
+    x = _rand(9, 64)
+    other = layers.densemx(64, 96).cuda()
+    with torch.no_grad():
+        want = other(x)
+        m = layers.densemx(64, 96).cuda().freeze()
+        assert not torch.equal(m(x), want)
+        m.load_state_dict(other.state_dict())
+        assert torch.equal(m(x), want) and torch.equal(m.freeze()(x), want)
+        for assign in (False, True):      # inside a larger module, too
+            net = torch.nn.Sequential(layers.densemx(64, 96).cuda().freeze()).eval()
+            net.load_state_dict({"0." + k: v.clone() for k, v in other.state_dict().items()}, assign=assign)
+            assert torch.equal(net(x), want)
+        m = layers.densemx(64, 96).cuda().freeze().cpu()
+        m.load_state_dict(other.state_dict())
+        assert torch.equal(m.cuda()(x), want)
+        m = layers.densemx(64, 96).cuda().freeze()
+        m.cpu()
+        m.kernel.copy_(other.kernel.cpu())
+        m.bias.copy_(other.bias.cpu())
+        assert torch.equal(m.cuda()(x), want)
+        m = layers.densemx(64, 96).cuda().freeze()
+        m.kernel, m.bias = other.kernel, other.bias
+        assert torch.equal(m(x), want)
+
+
+def test_gradients_through_a_frozen_layer():
+    from approxtrain_b200 import layers
+    m = layers.densemx(64, 96, activation="relu").cuda()
+    x, dy = _rand(9, 64), _rand(9, 96, seed=1)
+    leaves = [x.clone().requires_grad_(), m.kernel, m.bias]
+    y = m(leaves[0])
+    want = torch.autograd.grad(y, leaves, dy)
+    y2 = m.freeze()(leaves[0])
+    assert torch.equal(y2, y)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y2, leaves, dy), want))
+    # (with x's gradient unwanted the nine terms of a bias's gradient are added in another order: eight roundings in either)
+    alone = torch.autograd.grad(m(x), m.bias, dy)[0]
+    assert bool(((alone - want[2]).abs() <= 16 * 2.0 ** -24 * dy.abs().sum(0)).all())
+    m.requires_grad_(False)
+    assert torch.equal(torch.autograd.grad(m(leaves[0]), leaves[0], dy)[0], want[0])
+    assert torch.equal(m(x), y) and not m(x).requires_grad
