@@ -189,6 +189,7 @@ extern "C" int amsim_rotary(void* stream, const void* x, void* out, int heads, c
   if (batch >= (1ll << 31) || seq >= (1ll << 31) || (batch && seq > (1ll << 40) / batch)) return host_fail(AMSIM_ERR_UNSUPPORTED, "rotary: more than 2^31 sequences or positions");
   if (batch * seq == 0 || heads + heads2 == 0) return AMSIM_OK;
   if (!positions || !freqs || !strides || (heads && (!x || !out)) || (heads2 && (!x2 || !out2))) return host_fail(AMSIM_ERR_INVALID, "NULL tensor pointer");
+  if (heads && heads2 && out == out2) return host_fail(AMSIM_ERR_INVALID, "rotary: both tensors have the same output");
   rotary::Params p = {};
   const bool in_place = (!heads || x == out) && (!heads2 || x2 == out2);
   const bool half = !(flags & AMSIM_ROTARY_INTERLEAVED);

@@ -253,6 +253,40 @@ def _rotary_heads(x, name, like=None):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _share_elements(a, b) -> bool:
+    """Whether two tensors of one type share an element (True also where that takes long to tell).  A place that both have is a
+    solution of: sum of stride x difference of indices = distance between them; found from the longest stride down."""
+    span = {}   # stride -> least and largest difference of indices
+    for t, sign in ((a, 1), (b, -1)):
+        if not t.numel():
+            return False
+        for n, st in zip(t.shape, t.stride()):
+            if n > 1 and st:
+                lo, hi = span.get(st, (0, 0))
+                span[st] = (lo, hi + n - 1) if sign > 0 else (lo - n + 1, hi)
+    strides = sorted(span, reverse=True)
+    behind = [(0, 0)]   # what the strides behind each one reach
+    for st in strides[:0:-1]:
+        behind.insert(0, (behind[0][0] + st * span[st][0], behind[0][1] + st * span[st][1]))
+    left = {(b.data_ptr() - a.data_ptr()) // a.element_size()}
+    for st, (lo, hi) in zip(strides, behind):
+        ranges = [(d, max(span[st][0], -((hi - d) // st)), min(span[st][1], (d - lo) // st)) for d in left]
+        if sum(max(0, last - first + 1) for _, first, last in ranges) > 4096:
+            return True
+        left = {d - st * i for d, first, last in ranges for i in range(first, last + 1)}
+    return 0 in left
+
+
+def _repeats_elements(t) -> bool:
+    """Whether an element may have several places in t: where a stride is no longer than all that the shorter ones reach."""
+    reach = 0
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st <= reach:
+            return t.numel() > 0
+        reach += st * (n - 1)
+    return False
+
+
 def _strides(x):
     return (0, *x.stride()[:2]) if x.dim() == 3 else x.stride()[:3]
 
@@ -267,7 +301,7 @@ def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half",
     last axis (``transpose(1, 2)`` of [batch, heads, positions, dim], a slice of a joint projection); k may have other heads
     than q.  ``positions``: int32 or int64, [positions] or [batch, positions].  ``layout``: "half" (pairs half of the rotated
     part apart) or "interleaved" (adjacent).  The first ``freqs.rotary_dim`` elements of a head turn, the rest are
-    copied.  ``inverse`` turns back.  ``inplace`` writes over q and k.  Returns q's result, or both."""
+    copied.  ``inverse`` turns back.  ``inplace`` writes over q and k, which must not overlap.  Returns q's result, or both."""
     q = _rotary_heads(q, "q") if not inplace else _tensor(q, "q")
     k_ = None
     if k is not None:
@@ -276,11 +310,13 @@ def rotary(q, positions, freqs: RotaryFrequencies, k=None, layout: str = "half",
         for t, name in ((q, "q"), (k, "k")):
             if t is not None and t.shape[-1] != 1 and t.stride(-1) != 1:
                 raise ValueError(f"{name} must have a dense last axis to be rotated in place")
-            if t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-                raise ValueError(f"{name} must not be an expanded tensor to be rotated in place")
+            if t is not None and _repeats_elements(t):
+                raise ValueError(f"{name} must not be expanded or overlap itself to be rotated in place")
             if t is not None and t.requires_grad and torch.is_grad_enabled():
                 raise ValueError(f"{name} requires a gradient: it cannot be rotated in place (layers.rotary keeps gradients)")
         _rotary_heads(q, "q")
+        if k is not None and _share_elements(q, k):
+            raise ValueError("q and k must not share elements to be rotated in place")
     if not isinstance(freqs, RotaryFrequencies):
         raise TypeError("freqs must be RotaryFrequencies (rotary_frequencies)")
     if freqs.rotary_dim > q.shape[-1]:

@@ -172,3 +172,28 @@ def test_on_another_stream_and_in_a_graph():
     positions += 7
     graph.replay()
     assert torch.equal(out, ops.rotary(q, positions, freqs)) and not torch.equal(out, want)
+
+
+def test_in_place_beside_each_other_and_overlapping():
+    """Both tensors in place: parts of one projection are turned, tensors that share elements are refused as they are."""
+    from approxtrain_b200 import ops
+    freqs = ops.rotary_frequencies(32)
+    positions = torch.arange(9, device="cuda")
+    for t in (torch.float32, torch.bfloat16):
+        joint = _rand(2, 9, 8 * 48, t=t)
+        was = joint.clone()
+        heads = joint.unflatten(-1, (8, 48))
+        three = _rand(2, 9, 4 * 3 * 48, t=t, seed=1).unflatten(-1, (4, 3, 48))
+        for q, k in ((heads[:, :, :5], heads[:, :, 5:7]), (three[..., 0, :], three[..., 1, :])):
+            want = ops.rotary(q, positions, freqs, k=k)
+            got = ops.rotary(q, positions, freqs, k=k, inplace=True)
+            assert got[0] is q and got[1] is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+        assert torch.equal(heads[:, :, 7], was.unflatten(-1, (8, 48))[:, :, 7])
+        before = joint.clone()
+        for q, k in ((heads, heads), (heads[:, :, :5], heads[:, :, 4:]), (heads[:, :, ::2], heads[:, :, 2:4])):
+            with pytest.raises(ValueError, match="share"):
+                ops.rotary(q, positions, freqs, k=k, inplace=True)
+        with pytest.raises(ValueError, match="overlap"):
+            ops.rotary(joint.as_strided((9, 4, 48), (48, 48, 1)), positions, freqs, inplace=True)
+        assert torch.equal(joint, before)
+        assert all(torch.equal(x, y) for x, y in zip(ops.rotary(heads, positions, freqs, k=heads), [ops.rotary(heads, positions, freqs)] * 2))

@@ -176,3 +176,53 @@ def test_mx_refusals(L):
     assert m(None, p, p, 4, 4, 4, None, 0, p, 3) == L.ERR_INVALID and m(None, None, p, 4, 4, 4, None, 0, p, 0) == L.ERR_INVALID
     assert m(None, p + 8, p, 4, 4, 4, None, 0, p, 0) == L.ERR_INVALID and m(None, p, p, 1 << 30, 1 << 30, 4, None, 0, p, 0) == L.ERR_UNSUPPORTED
     assert m(None, p, p, 0, 4, 4, None, 0, p, 0) == 0
+
+
+def test_tensors_that_overlap_are_told_from_those_that_do_not():
+    import random
+    from approxtrain_b200.train_ops import _repeats_elements, _share_elements
+    buf = torch.zeros(4000)
+    rng = random.Random(5)
+
+    def places(t):
+        at = torch.tensor(t.storage_offset())
+        for n, st in zip(t.shape, t.stride()):
+            at = at[..., None] + st * torch.arange(n)
+        return at.flatten().tolist()
+
+    def view():
+        shape = [rng.randrange(1, 4) for _ in range(4)]
+        strides = [rng.choice([0, 1, 2, 3, 5, 8, 12, 24, 40, 60]) for _ in range(4)]
+        return buf.as_strided(shape, strides, rng.randrange(0, 120))
+    shared = apart = 0
+    for _ in range(3000):
+        a, b = view(), view()
+        both = bool(set(places(a)) & set(places(b)))
+        assert _share_elements(a, b) == both == _share_elements(b, a)
+        shared, apart = shared + both, apart + (not both)
+        assert _repeats_elements(a) or len(set(places(a))) == a.numel()
+    assert shared > 300 and apart > 300
+    # what a model hands over: parts of one projection, by head or interleaved, and of one buffer
+    joint = torch.zeros(2, 9, 3 * 4 * 48)
+    q, k = joint[..., :192].unflatten(-1, (4, 48)), joint[..., 192:288].unflatten(-1, (2, 48))
+    assert not _share_elements(q, k) and not _repeats_elements(q) and _share_elements(q, joint[..., 144:240].unflatten(-1, (2, 48)))
+    three = joint.unflatten(-1, (4, 3, 48))
+    assert not _share_elements(three[..., 0, :], three[..., 1, :]) and _share_elements(three[..., 1, :], three[..., 1, :])
+    flat = torch.zeros(2 * 6 * 9 * 48)
+    q, k = flat[:2 * 4 * 9 * 48].view(2, 4, 9, 48).transpose(1, 2), flat[2 * 4 * 9 * 48:].view(2, 2, 9, 48).transpose(1, 2)
+    assert not _share_elements(q, k) and not _repeats_elements(q) and not _repeats_elements(k)
+    assert not _share_elements(q[:0], q) and not _repeats_elements(q[:0])
+    assert _repeats_elements(flat.as_strided((3, 5, 2, 8), (0, 8, 4, 1))) and _repeats_elements(flat[:48].expand(9, 4, 48))
+    # (strides that make it a long search count as shared)
+    wide = torch.zeros(1).as_strided((1, 1, 1, 1), (1, 1, 1, 1))
+    assert not _share_elements(wide, torch.zeros(1, 1, 1, 1))
+
+
+def test_rotary_of_one_output_twice_is_refused(L):
+    p = 1 << 20
+    strides = (C.c_longlong * 14)(64, 16, 8, 64, 16, 8, 64, 16, 8, 64, 16, 8, 0, 1)
+
+    def call(x2, out2):
+        return L.lib.amsim_rotary(None, p, p, 2, x2, out2, 2, p, p, 1, 4, 8, 8, strides, 1.0, 0, 0)
+    assert call(p, p) == L.ERR_INVALID and b"same output" in L.lib.amsim_last_error()
+    assert call(2 * p, p) == L.ERR_INVALID
