@@ -242,5 +242,6 @@ class DataParallelAdamW(DataParallelSGD):
         return {"lr": self.lr, "moments": self.state.state_dict()}
 
     def load_state_dict(self, state: dict) -> None:
-        self.set_lr(state["lr"])
+        lr = float(state["lr"])
         self.state.load_state_dict(state["moments"])
+        self.set_lr(lr)

@@ -411,13 +411,15 @@ class AdamWState:
         return {"bits": self.bits, "shapes": list(self.shapes), "step": self.step.clone(), **{k: getattr(self, k).clone() for k in self._moments}}
 
     def load_state_dict(self, state: dict) -> None:
+        """Takes over what ``state_dict`` gave; a state that does not fit is refused and nothing is changed."""
         if state["bits"] != self.bits or [tuple(s) for s in state["shapes"]] != self.shapes:
             raise ValueError("the state is of other parameters or other bits")
+        step = int(state["step"])
+        for k in self._moments:
+            if state[k].shape != getattr(self, k).shape or state[k].dtype != getattr(self, k).dtype:
+                raise ValueError(f"{k} does not match")
         with torch.no_grad():
-            self._counter[0] = state["step"].to(self.device)
-            for k in self._moments:
-                if state[k].shape != getattr(self, k).shape or state[k].dtype != getattr(self, k).dtype:
-                    raise ValueError(f"{k} does not match")
+            self._counter[0] = step
             for k in self._moments:
                 getattr(self, k).copy_(state[k])
 

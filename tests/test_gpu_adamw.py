@@ -288,3 +288,27 @@ def test_trainer():
                     # a first step is lr * g / (|g| + eps): at most lr, with a dozen roundings of it and one of p on either side
                     assert float((a - b).detach().abs().max()) <= 32 * F32 * (1e-3 + float(b.detach().abs().max()))
         assert losses[0] == losses[1]
+
+
+def test_a_state_that_is_refused_changes_nothing():
+    from approxtrain_b200 import ops
+    from approxtrain_b200.dp import DataParallelAdamW
+    for bits in (32, 8):
+        net = torch.nn.Linear(30, 20).cuda()
+        tr = DataParallelAdamW(net, 1e-3, state_bits=bits)
+        x = torch.randn(4, 30, device="cuda")
+        tr.step(lambda: net(x).square().sum())
+        tr.step(lambda: net(x).square().sum())
+        was = tr.state.state_dict()
+        other = DataParallelAdamW(torch.nn.Linear(30, 20).cuda(), 5e-2, state_bits=bits).state_dict()
+        for spoil in (lambda m: m.update(exp_avg=m["exp_avg"][1:]), lambda m: m.pop(tr.state._moments[-1]), lambda m: m.pop("step"),
+                      lambda m: m.update({tr.state._moments[-1]: m[tr.state._moments[-1]].half()}), lambda m: m.update(bits=16), lambda m: m.update(shapes=[(1,)])):
+            bad = dict(other, moments=dict(other["moments"]))
+            spoil(bad["moments"])
+            with pytest.raises((ValueError, KeyError)):
+                tr.load_state_dict(bad)
+            now = tr.state.state_dict()
+            assert tr.lr == 1e-3 and float(tr._lr) == pytest.approx(1e-3) and int(tr.state.step) == 2
+            assert all(torch.equal(now[k].float(), was[k].float()) for k in tr.state._moments)
+        tr.load_state_dict(other)
+        assert tr.lr == 5e-2 and int(tr.state.step) == 0 and not tr.state.moments(0)[0].any()
