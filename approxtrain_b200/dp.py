@@ -214,7 +214,7 @@ class DataParallelSGD:
 class DataParallelAdamW(DataParallelSGD):
     """The same trainer with AdamW (``ops.adamw_step``) as the replicated update: one launch over all parameters, moments in 32
     bits or in 8 (``state_bits``), on CUDA devices.  The step count and the learning rate live on the device, so a captured step
-    (``capture``) counts on and follows ``set_lr`` when it is replayed.  Every rank rounds 8-bit moments with the same
+    (``capture``) counts on and follows ``trainer.lr = x`` (or ``set_lr(x)``) when it is replayed.  Every rank rounds 8-bit moments with the same
     `seed`: replicas stay identical.  Parameters of one axis (biases, norms) get no weight decay."""
 
     _ALIGN = 4   # gradients on 16-byte boundaries
@@ -228,9 +228,18 @@ class DataParallelAdamW(DataParallelSGD):
         self.state = ops.AdamWState(self.params, bits=state_bits)
         self._lr = torch.full((1,), lr, dtype=torch.float32, device=self.state.device)
 
+    @property
+    def lr(self) -> float:
+        return self._rate
+
+    @lr.setter
+    def lr(self, lr: float) -> None:
+        self._rate = lr
+        if hasattr(self, "_lr"):
+            self._lr.fill_(lr)
+
     def set_lr(self, lr: float) -> None:
         self.lr = lr
-        self._lr.fill_(lr)
 
     def _update(self):
         from . import ops

@@ -312,3 +312,30 @@ def test_a_state_that_is_refused_changes_nothing():
             assert all(torch.equal(now[k].float(), was[k].float()) for k in tr.state._moments)
         tr.load_state_dict(other)
         assert tr.lr == 5e-2 and int(tr.state.step) == 0 and not tr.state.moments(0)[0].any()
+
+
+def test_the_rate_of_a_trainer_is_the_one_that_is_set():
+    """``trainer.lr = x`` as with the other trainer, for eager and for captured steps."""
+    from approxtrain_b200.dp import DataParallelAdamW
+    x = torch.randn(16, 30, device="cuda")
+    finals = []
+    for captured in (False, True):
+        torch.manual_seed(1)
+        net = torch.nn.Linear(30, 20).cuda()
+        tr = DataParallelAdamW(net, 1e-3, weight_decay=0.0)
+        loss_fn = lambda: net(x).square().sum()
+        step = tr.capture(loss_fn, warmup=3) if captured else lambda: tr.step(loss_fn)
+        for _ in range(0 if captured else 3):
+            step()
+        tr.lr = 0.0
+        before = net.weight.detach().clone()
+        step()
+        assert torch.equal(net.weight, before) and tr.lr == 0.0
+        tr.lr = 0.25
+        step()
+        assert float((net.weight - before).detach().abs().max()) > 0.1 and tr.state_dict()["lr"] == 0.25
+        tr.set_lr(0.5)
+        assert tr.lr == 0.5
+        step()
+        finals.append(net.weight.detach().clone())
+    assert torch.equal(*finals)
