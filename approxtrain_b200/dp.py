@@ -67,10 +67,11 @@ class DataParallelSGD:
                 p.amsim_grad_sink = GradSink(p.grad, hook)
                 self._sinks.append(p.amsim_grad_sink)
 
-    _ALIGN = 1   # elements a gradient's place in its bucket is a multiple of
+    _ALIGN_BYTES = 1   # a gradient's place in its bucket is a multiple of so many
 
     def _close_bucket(self, params):
-        room = [-(-p.numel() // self._ALIGN) * self._ALIGN for p in params]
+        align = max(1, self._ALIGN_BYTES // params[0].element_size())
+        room = [-(-p.numel() // align) * align for p in params]
         flat = torch.zeros(sum(room), dtype=params[0].dtype, device=params[0].device)
         off = 0
         for p, n in zip(params, room):
@@ -217,7 +218,7 @@ class DataParallelAdamW(DataParallelSGD):
     (``capture``) counts on and follows ``trainer.lr = x`` (or ``set_lr(x)``) when it is replayed.  Every rank rounds 8-bit moments with the same
     `seed`: replicas stay identical.  Parameters of one axis (biases, norms) get no weight decay."""
 
-    _ALIGN = 4   # gradients on 16-byte boundaries
+    _ALIGN_BYTES = 16   # the step reads such gradients 16 bytes at a time, or four 16-bit elements
 
     def __init__(self, model: torch.nn.Module, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, seed: int = 0, bucket_bytes: int = 32 << 20, process_group=None):

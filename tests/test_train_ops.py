@@ -226,3 +226,22 @@ def test_rotary_of_one_output_twice_is_refused(L):
         return L.lib.amsim_rotary(None, p, p, 2, x2, out2, 2, p, p, 1, 4, 8, 8, strides, 1.0, 0, 0)
     assert call(p, p) == L.ERR_INVALID and b"same output" in L.lib.amsim_last_error()
     assert call(2 * p, p) == L.ERR_INVALID
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_of_the_adamw_trainer_begin_at_16_bytes(t):
+    from approxtrain_b200.dp import DataParallelAdamW, DataParallelSGD
+    sizes = [1, 5, 12, 4, 7, 300]
+    for cls in (DataParallelAdamW, DataParallelSGD):
+        tr = object.__new__(cls)
+        tr.buckets = []
+        params = [torch.nn.Parameter(torch.zeros(n, dtype=t)) for n in sizes]
+        tr._close_bucket(params)
+        flat = tr.buckets[0]["flat"]
+        at = [(p.grad.data_ptr() - flat.data_ptr()) for p in params]
+        if cls is DataParallelAdamW:
+            assert all(a % 16 == 0 for a in at)
+        else:
+            assert flat.numel() == sum(sizes)
+        ends = [a + n * flat.element_size() for a, n in zip(at, sizes)]
+        assert all(e <= a for e, a in zip(ends, at[1:])) and ends[-1] <= flat.numel() * flat.element_size()
