@@ -89,8 +89,8 @@ __device__ __forceinline__ float load1(const void* base, long long i) { return e
 template <typename T>
 __device__ __forceinline__ void store1(void* base, long long i, float v) { static_cast<T*>(base)[i] = elem_from_float<T>(v); }
 
-// FP32 moments: 8 elements of a thread at a time, twice four adjacent ones (VEC), or each beside its neighbour thread's.  (16 spill at 128
-// registers, 8 keep 96 KB of a multiprocessor in flight.)
+// FP32 moments: 8 elements of a thread at a time, twice four adjacent ones (VEC), or each beside its neighbour thread's.  (8 at
+// 80 registers, 52 to 60 bytes of them spilled, keep 96 KB of a multiprocessor in flight.)
 template <typename TP, typename TG, bool VEC>
 __device__ __forceinline__ void half_chunk32(const Entry& e, const Common& c, long long base, const Rates& r) {
   float* const m_at = static_cast<float*>(c.m) + e.at;
@@ -351,7 +351,7 @@ __device__ __forceinline__ int find(const Table<CAP>& tab, long long unit) {
 }
 
 // 56 million parameters in 244 tensors: FP32 moments 260 us (6.1 TB/s), 8 bits 207 us (4.4 TB/s), bound by the issue of
-// instructions (84 a parameter, two of three issue slots taken).
+// instructions: 84 a parameter, 65 % of the issue slots, which 16 warps a multiprocessor (114 to 120 registers) do not fill.
 template <typename TP, typename TG, int BITS, int CAP>
 __global__ void __launch_bounds__(THREADS, BITS == 32 ? 3 : 2) adamw(const __grid_constant__ Table<CAP> tab) {
   __shared__ Rates rates;

@@ -8,7 +8,7 @@
 // Both are bound by memory: the forward pass reads x and block and writes y (and r where it is wanted); the backward pass
 // reads dy, dr, x and block, from which it makes r and hat again, unrounded (taken from a stored bf16 r, the gradients of the FP32 weights
 // were 1.6e-3 off), and writes dx and dblock.  A row stays in registers from its one read to its one write: `tpr` threads
-// (a power of two from 4 to 512) hold E elements each; rows wider than a CTA's share go to a cluster of 2, 4 or 8 CTAs
+// (4, 8, 16 or a multiple of 32 up to 512) hold E elements each; rows wider than a CTA's share go to a cluster of 2, 4 or 8 CTAs
 // that add their row sums through distributed shared memory.  What a thread will need of its next rows is already on
 // its way to a place of its own in shared memory (cp.async, no barrier), since the chain of two or four row sums per row
 // leaves the memory idle otherwise.  Means, variances and every sum are FP32 (a variance around the thread's own mean, joined in pairs);
@@ -305,7 +305,7 @@ struct Walk {
 };
 
 // Forward.  8192 x 512 FP32, x + block and a layer norm: 11.7 us (4.3 TB/s; 50 MB from and to memory).  16384 x 2048 bf16 with both
-// rms norms, a gate per sequence and the sum written: 59 us (4.6 TB/s), issuing instructions half of the time.
+// rms norms, a gate per sequence and the sum written: 59 us (4.6 TB/s), 57 % of the issue slots and 44 % of DRAM: latency, as below.
 template <typename T, int V, bool LAYER, bool POST, int GATE, int E, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_fwd(const __grid_constant__ NormParams p) {
   constexpr int N = E / V;
@@ -447,8 +447,9 @@ __device__ __forceinline__ void flush_block(float (&acc)[N][V], const Cols<V, FU
   }
 }
 
-// Backward.  The same cases: 14.7 us (4.6 TB/s) and 5.1 us of norm_reduce; 120 us (3.3 TB/s) and 6 us.  The second is bound by the issue of
-// instructions, about 70 an element: conversions, 28 of arithmetic, and a row's fixed share (two row sums, addresses) over 8 elements.
+// Backward.  The same cases: 14.7 us (4.6 TB/s) and 5.1 us of norm_reduce; 120 us (3.3 TB/s) and 6 us.  The second is bound by latency: 54 % of
+// the issue slots and 37 % of DRAM, with 16 warps a multiprocessor (118 registers), each in a chain of two row sums a row; about 70 instructions
+// an element (conversions, 28 of arithmetic, and a row's fixed share over 8 elements) leave little to hide it behind.
 template <typename T, int V, bool LAYER, bool POST, int GATE, int E, bool FULL>
 __global__ void __launch_bounds__(MAX_THREADS) norm_bwd(const __grid_constant__ NormParams p) {
   constexpr int N = E / V;

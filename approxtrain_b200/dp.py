@@ -158,7 +158,9 @@ class DataParallelSGD:
         the per-launch host cost of the several hundred small exact kernels around the AM ops
         (normalisation, activations, pooling, bias gradients), which is what bounds the launch-bound
         LeNet configurations and costs the large networks a few percent.  The tensors ``loss_fn``
-        reads must be static (copy new batches into them).
+        reads must be static (copy new batches into them).  No autograd graph of an earlier loss of the same
+        parameters may be alive while it records: torch ties a parameter's gradient to the stream of the first
+        graph that uses it, and refuses to capture another.
 
         Single process: one graph holds zero-grads, forward, backward and the SGD update.
         With a process group: one graph holds zero-grads, forward and backward; the gradient

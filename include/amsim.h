@@ -393,8 +393,9 @@ unsigned long long amsim_debug_launch_count(void);
 void amsim_debug_reload_env(void);
 
 /* Bounds-checking debug build (compiled with -DAMSIM_BOUNDS_CHECK; the stand-in for a device-side
- * memory checker): every access of the kernels to a caller's tensor or to scratch is compared with
- * the buffer's extent and alignment before it is made; a bad one is skipped and the first is
+ * memory checker): every access of the convolution, dense and matmul
+ * kernels to a caller's tensor or to scratch is compared with the buffer's extent and alignment before it is made (kernels with
+ * one-to-one index maps, and those of the norms, rotary positions, AdamW and the 4-bit products, are not instrumented); a bad one is skipped and the first is
  * recorded.  This call waits for the device, returns that record in *word (0 = every access since
  * the last call was in bounds; otherwise source line << 44 | (buffer + 1) << 40 | byte offset, buffers
  * 0 lane operand, 1 uniform operand, 2 output, 3 scratch) and clears it.  A normal build returns
@@ -403,8 +404,8 @@ int amsim_debug_bounds_report(unsigned long long* word);
 
 /* The tensor-core kernels bound every wait between their warps; one that runs out makes the kernel
  * end with wrong results instead of hanging (it never should).  The kernel leaves a mark in host
- * memory, and the next call that takes a LUT on that device returns AMSIM_ERR_CUDA once, launching
- * nothing.  amsim_async_status does nothing else: AMSIM_OK, or that error, without waiting for the
+ * memory, and the next call that takes a LUT, or the next amsim_mx_matmul, on that device returns
+ * AMSIM_ERR_CUDA once, launching nothing.  amsim_async_status does nothing else: AMSIM_OK, or that error, without waiting for the
  * device (for hosts that replay captured launches and make no other calls).
  * amsim_debug_wait_report waits for the device, returns nonzero in *stuck if it has happened on
  * the current device since it was last reported, and clears the mark.  No reference counterpart. */
