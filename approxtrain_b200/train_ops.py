@@ -256,10 +256,13 @@ def _rotary_heads(x, name, like=None):
 def _share_elements(a, b) -> bool:
     """Whether two tensors of one type share an element (True also where that takes long to tell).  A place that both have is a
     solution of: sum of stride x difference of indices = distance between them; found from the longest stride down."""
+    if not a.numel() or not b.numel():
+        return False
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if a.is_contiguous() and b.is_contiguous():
+        return -b.numel() < apart < a.numel()
     span = {}   # stride -> least and largest difference of indices
     for t, sign in ((a, 1), (b, -1)):
-        if not t.numel():
-            return False
         for n, st in zip(t.shape, t.stride()):
             if n > 1 and st:
                 lo, hi = span.get(st, (0, 0))
@@ -268,7 +271,7 @@ def _share_elements(a, b) -> bool:
     behind = [(0, 0)]   # what the strides behind each one reach
     for st in strides[:0:-1]:
         behind.insert(0, (behind[0][0] + st * span[st][0], behind[0][1] + st * span[st][1]))
-    left = {(b.data_ptr() - a.data_ptr()) // a.element_size()}
+    left = {apart}
     for st, (lo, hi) in zip(strides, behind):
         ranges = [(d, max(span[st][0], -((hi - d) // st)), min(span[st][1], (d - lo) // st)) for d in left]
         if sum(max(0, last - first + 1) for _, first, last in ranges) > 4096:
